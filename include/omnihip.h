@@ -15,8 +15,8 @@
  *   - return value 0 = launched; non-zero = rejected before any launch, with the reason
  *     in ovd_last_error() (thread-local, valid until the next call on that thread);
  *   - strides (`ld*`, `*_bs`) are in ELEMENTS;
- *   - two helpers do no GPU work and are marked HOST at their declaration
- *     (ovd_resize_coeffs fills host tables, ovd_flash_attn_workspace_bytes returns a size).
+ *   - a few helpers do no GPU work and are marked HOST at their declaration
+ *     (ovd_resize_coeffs fills host tables, the others return a size).
  */
 #ifndef OMNIHIP_H
 #define OMNIHIP_H
@@ -301,6 +301,31 @@ int ovd_flash_attn_qk8_fwd_bf16(const int8_t* q8, const float* q_scale, const in
                                 int64_t q_ld, int64_t k_ld, int64_t v_ld, int64_t o_ld, int64_t q_bs, int64_t k_bs,
                                 int64_t v_bs, int64_t o_bs, float softmax_scale, void* workspace,
                                 int64_t workspace_bytes, void* stream);
+
+/* ---- MXFP4 (OCP microscaling: E2M1 elements, one E8M0 scale per 32 consecutive values of a row) form of the
+ * linear layers.  No reference counterpart (bf16 there: omnivideo/modules/model.py:125-154, :159-179, :218-258).
+ *
+ * A matrix [rows, K] is held as two buffers of ovd_mxfp4_data_bytes / ovd_mxfp4_scale_bytes (HOST functions) bytes,
+ * in the order in which the matrix instructions read them (Kp = K rounded up to 256, lane = 32 h + r):
+ *   data  [ceil(rows/32)][Kp/64][64 lanes][16]: the codes of row 32 rb + r, k = 64 kt + 32 h .. + 31, low nibble first;
+ *   scale [ceil(rows/32)][Kp/256][64 lanes][4]: byte j = the scale byte of that lane's block in k-step 4 kg + j.
+ * data must be 16-byte aligned, scale 4-byte aligned; each call writes everything of the rows it is given, and bytes
+ * of rows past the last one are neither written nor used.
+ *
+ * ovd_mxfp4_quant: x [M, K] (fp32 when x_is_f32, else bf16; rows 16-byte aligned), K % 32 == 0.  Scale byte of a block
+ *   s = max(floor(log2 max|x|) + 125, 0), 255 when the block holds an infinity or NaN (all its values then are NaN);
+ *   codes = x / 2^(s - 127) to the nearest E2M1 number, ties to even, saturated at 6.
+ * ovd_mxfp4_dequant: the values code * 2^(s - 127) as bf16 or fp32 (exact in both).
+ * ovd_gemm_mxfp4: out = epilogue(A[M,K] * W[N,K]^T + bias[N]) with fp32 accumulation; epilogue 0: bf16 out,
+ *   1: bf16 out of tanh-GELU, 2: fp32 out, 3: fp32 in-place out += y * gate[n] (gate NULL = 1).  One rounding, of the
+ *   stored value.  N % 4 == 0, K % 32 == 0, ldo % 4 == 0; bias bf16 [N] or NULL.  Sums are in a fixed order. */
+int64_t ovd_mxfp4_data_bytes(int64_t rows, int64_t K);
+int64_t ovd_mxfp4_scale_bytes(int64_t rows, int64_t K);
+int ovd_mxfp4_quant(const void* x, int x_is_f32, int64_t ldx, uint8_t* data, uint8_t* scale, int M, int K, void* stream);
+int ovd_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out, int out_is_f32, int64_t ldo, int M, int K,
+                      void* stream);
+int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
+                   void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream);
 
 /* Source-video frames -> VAE encoder input, the device half of transform_frames_to_tensor
  * (tools/inference/generate_omni_v2v.py:306-343: CenterCrop, Resize on a PIL image = Pillow's 8-bit

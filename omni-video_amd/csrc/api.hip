@@ -40,6 +40,12 @@ int ovd_impl_ln_fp8(float*, long, const bf16_t*, long, const float*, const float
                     const bf16_t*, uint8_t*, long, float*, int, int, float, int, hipStream_t);
 int ovd_impl_gemm_fp8(const uint8_t*, long, const float*, float, const uint8_t*, long, const float*, const bf16_t*, void*,
                       long, const float*, float, int, int, int, int, hipStream_t);
+long ovd_impl_mxfp4_data_bytes(long, long);
+long ovd_impl_mxfp4_scale_bytes(long, long);
+int ovd_impl_mxfp4_quant(const void*, int, long, uint8_t*, uint8_t*, int, int, hipStream_t);
+int ovd_impl_mxfp4_dequant(const uint8_t*, const uint8_t*, void*, int, long, int, int, hipStream_t);
+int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
+                        const float*, int, int, int, int, hipStream_t);
 int ovd_impl_frames_resize(const uint8_t*, uint8_t*, float*, const int*, const int*, int, const int*, const int*, int,
                            const float*, long, int, int, int, int, int, int, int, int, hipStream_t);
 int ovd_impl_t5_attention(const bf16_t*, long, const bf16_t*, const int*, const int*, bf16_t*, long, int, int, int, int,
@@ -321,6 +327,26 @@ int ovd_gemm_fp8(const uint8_t* A, int64_t lda, const float* a_scale, float a_sc
     NONNULL(A); NONNULL(W); NONNULL(w_scale); NONNULL(out);
     return ovd_impl_gemm_fp8(A, lda, a_scale, a_scale_all, W, ldw, w_scale, (const bf16_t*)bias, out, ldo, gate,
                              out_scale, M, N, K, epilogue, ST(stream));
+}
+
+int64_t ovd_mxfp4_data_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? 0 : ovd_impl_mxfp4_data_bytes(rows, K); }
+int64_t ovd_mxfp4_scale_bytes(int64_t rows, int64_t K) { return rows < 0 || K <= 0 ? 0 : ovd_impl_mxfp4_scale_bytes(rows, K); }
+
+int ovd_mxfp4_quant(const void* x, int x_is_f32, int64_t ldx, uint8_t* data, uint8_t* scale, int M, int K, void* stream) {
+    NONNULL(x); NONNULL(data); NONNULL(scale);
+    return ovd_impl_mxfp4_quant(x, x_is_f32, ldx, data, scale, M, K, ST(stream));
+}
+
+int ovd_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out, int out_is_f32, int64_t ldo, int M, int K,
+                      void* stream) {
+    NONNULL(data); NONNULL(scale); NONNULL(out);
+    return ovd_impl_mxfp4_dequant(data, scale, out, out_is_f32, ldo, M, K, ST(stream));
+}
+
+int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
+                   void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream) {
+    NONNULL(A); NONNULL(a_scale); NONNULL(W); NONNULL(w_scale); NONNULL(out);
+    return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, ST(stream));
 }
 
 int ovd_resize_coeffs(int in_size, int out_size, int* bounds_host, int* coef_host, int ksize_cap) {

@@ -47,6 +47,11 @@ SIGNATURES = {
     "ovd_quant_rows_fp8": [_p, _l, _p, _l, _p, _i, _i, _p],
     "ovd_layernorm_modulate_fp8": [_p, _l, _p, _p, _p, _p, _p, _l, _p, _i, _i, _f, _i, _p],
     "ovd_gemm_fp8": [_p, _l, _p, _f, _p, _l, _p, _p, _p, _l, _p, _f, _i, _i, _i, _i, _p],
+    "ovd_mxfp4_data_bytes": [_l, _l],
+    "ovd_mxfp4_scale_bytes": [_l, _l],
+    "ovd_mxfp4_quant": [_p, _i, _l, _p, _p, _i, _i, _p],
+    "ovd_mxfp4_dequant": [_p, _p, _p, _i, _l, _i, _i, _p],
+    "ovd_gemm_mxfp4": [_p, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _p],
     "ovd_resize_coeffs": [_i, _i, _p, _p, _i],
     "ovd_frames_resize_normalize": [_p, _p, _p, _p, _p, _i, _p, _p, _i, _p, _l, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "ovd_t5_attention_bf16": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _i, _p],
@@ -72,6 +77,8 @@ SIGNATURES = {
     "ovd_peer_sum_f32": [_p, _p, _l, _i, _p],
 }
 
+SIZE_FUNCTIONS = ("ovd_flash_attn_workspace_bytes", "ovd_mxfp4_data_bytes", "ovd_mxfp4_scale_bytes")      # return int64
+
 EPI_BF16, EPI_BF16_GELU, EPI_F32, EPI_RESID = 0, 1, 2, 3
 UNIPC_COEF_STRIDE = 16
 DPM_COEF_STRIDE = 8
@@ -91,7 +98,7 @@ def lib():
         for name, args in SIGNATURES.items():
             fn = getattr(L, name)
             fn.argtypes = args
-            fn.restype = _l if name == "ovd_flash_attn_workspace_bytes" else _i
+            fn.restype = _l if name in SIZE_FUNCTIONS else _i
         _lib = L
     return _lib
 
@@ -667,6 +674,90 @@ def gemm_fp8(a8, w8, w_scale, out, bias=None, epilogue=EPI_BF16, a_scale=None, a
     _call("ovd_gemm_fp8", _u8(a8), a8.stride(0), _f32c(a_scale, True), float(a_scale_all), _u8(w8), w8.stride(0),
           _f32c(w_scale), _ptr(bias, BF16, True), out.data_ptr(), out.stride(0), _f32c(gate, True), float(out_scale),
           M, N, K, epilogue, _stream())
+    return out
+
+
+# ---------------------------------------------------------------------------- MXFP4
+
+def _call_on(device, name, *args):
+    """_call with `device` current, on that device's current stream (appended as the last argument)."""
+    if device.index == torch.cuda.current_device():
+        _call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            _call(name, *args, _stream())
+
+
+def _one_device(*tensors):
+    """The HIP device that all given tensors (None skipped) are on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("libomnihip works on device tensors only (got a CPU tensor)")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"tensors are on different devices ({dev}, {t.device})")
+        dev = t.device
+    return dev
+
+
+def mxfp4_bytes(rows, cols):
+    """(bytes of codes, bytes of scales) of an MXFP4 matrix [rows, cols]."""
+    if rows < 0 or cols <= 0 or cols % 32:
+        raise ValueError(f"mxfp4: a [{rows}, {cols}] matrix has no blocks of 32")
+    L = lib()
+    return int(L.ovd_mxfp4_data_bytes(rows, cols)), int(L.ovd_mxfp4_scale_bytes(rows, cols))
+
+
+def _mx_operand(m):
+    nd, ns = mxfp4_bytes(m.rows, m.cols)
+    for t, n in ((m.data, nd), (m.scale, ns)):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < n:
+            raise ValueError(f"mxfp4: the buffers do not hold a [{m.rows}, {m.cols}] matrix")
+    return m.data.data_ptr(), m.scale.data_ptr()
+
+
+def mxfp4_quant(x, m):
+    """x bf16 / fp32 [M, K] (rows 16-byte aligned) -> m (MXFP4 matrix of that shape)."""
+    M, K = x.shape
+    if (m.rows, m.cols) != (M, K) or x.dtype not in (BF16, F32) or (K > 1 and x.stride(1) != 1):
+        raise ValueError("mxfp4: needs bf16 or fp32 rows of the matrix's shape")
+    dev = _one_device(x, m.data, m.scale)
+    d, s = _mx_operand(m)
+    if M:
+        _call_on(dev, "ovd_mxfp4_quant", x.data_ptr(), int(x.dtype == F32), x.stride(0) if M > 1 else K, d, s, M, K)
+    return m
+
+
+def mxfp4_dequant(m, out):
+    if tuple(out.shape) != (m.rows, m.cols) or out.dtype not in (BF16, F32) or (m.cols > 1 and out.stride(1) != 1):
+        raise ValueError("mxfp4: out must be bf16 or fp32 rows of the matrix's shape")
+    dev = _one_device(out, m.data, m.scale)
+    d, s = _mx_operand(m)
+    if m.rows:
+        _call_on(dev, "ovd_mxfp4_dequant", d, s, out.data_ptr(), int(out.dtype == F32),
+                 out.stride(0) if m.rows > 1 else m.cols, m.rows, m.cols)
+    return out
+
+
+def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
+    """out = epilogue(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; out [..., N] with a uniform row stride."""
+    M, N, K = a.rows, w.rows, a.cols
+    if w.cols != K or out.numel() != M * N or out.shape[-1] != N:
+        raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}] out{tuple(out.shape)}")
+    want = BF16 if epilogue in (EPI_BF16, EPI_BF16_GELU) else F32
+    for v, dt in ((bias, BF16), (gate, F32)):
+        if v is not None and (v.numel() != N or not v.is_contiguous() or v.dtype != dt):
+            raise ValueError(f"gemm_mxfp4: bias (bf16) and gate (fp32) must be contiguous rows of length {N}")
+    if out.dtype != want:
+        raise TypeError(f"gemm_mxfp4: this epilogue writes {want}, out is {out.dtype}")
+    dev = _one_device(a.data, a.scale, w.data, w.scale, out, bias, gate)
+    (ad, asc), (wd, wsc) = _mx_operand(a), _mx_operand(w)
+    if M:
+        _, _, ldo = _rows(out)
+        _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                 ldo if M > 1 else N, None if gate is None else gate.data_ptr(), M, N, K, epilogue)
     return out
 
 

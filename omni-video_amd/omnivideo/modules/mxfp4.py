@@ -1,0 +1,127 @@
+"""Linear layers on MXFP4 operands (OCP microscaling: 4-bit E2M1 elements, one power-of-two scale per 32 consecutive
+values of a row): an extension beside the e4m3 mode, for layers the reference runs as bf16 nn.Linear
+(omnivideo/modules/model.py:125-154, :159-179, :218-258).  Backed by ovd_mxfp4_quant, ovd_mxfp4_dequant and
+ovd_gemm_mxfp4.  Inference only: the results carry no gradient."""
+import torch
+
+from .. import _hip as H
+
+__all__ = ["MXFP4Matrix", "mxfp4_quantize", "mxfp4_linear"]
+
+BF16, F32, U8 = torch.bfloat16, torch.float32, torch.uint8
+
+
+class MXFP4Matrix:
+    """A [rows, cols] matrix in MXFP4, its codes and scales in the order in which the matrix instructions read them
+    (include/omnihip.h).  Made by `mxfp4_quantize` or `from_ocp`; a layer's weights are laid out once."""
+
+    def __init__(self, rows, cols, data, scale):
+        self.rows, self.cols, self.data, self.scale = rows, cols, data, scale
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @classmethod
+    def empty(cls, rows, cols, device):
+        """Uninitialised storage for a [rows, cols] matrix (cols a multiple of 32)."""
+        nd, ns = H.mxfp4_bytes(rows, cols)
+        return cls(rows, cols, torch.empty(nd, dtype=U8, device=device), torch.empty(ns, dtype=U8, device=device))
+
+    @classmethod
+    def from_ocp(cls, codes, scales):
+        """From the row-major form of checkpoints: codes uint8 [rows, cols / 2] (k ascending, low nibble first) and
+        E8M0 scale bytes uint8 [rows, cols / 32]."""
+        if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != U8 or scales.dtype != U8:
+            raise TypeError("MXFP4: codes and scales must be two-dimensional uint8 tensors")
+        rows, cols = codes.shape[0], 2 * codes.shape[1]
+        if rows == 0 or cols == 0 or cols % 32 or tuple(scales.shape) != (rows, cols // 32):
+            raise ValueError(f"MXFP4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not describe a "
+                             "matrix with blocks of 32")
+        if codes.device != scales.device:
+            raise ValueError("MXFP4: codes and scales are on different devices")
+        rb, kg = -(-rows // 32), -(-cols // 256)
+        c = codes.new_zeros(rb * 32, kg * 128)
+        c[:rows, :cols // 2] = codes
+        s = scales.new_zeros(rb * 32, kg * 8)
+        s[:rows, :cols // 32] = scales
+        # [rb, r, kt, h, 16 bytes] -> [rb, kt, h, r, 16];  [rb, r, kg, ks, h] -> [rb, kg, h, r, ks]
+        data = c.view(rb, 32, kg * 4, 2, 16).permute(0, 2, 3, 1, 4).contiguous()
+        scale = s.view(rb, 32, kg, 4, 2).permute(0, 2, 4, 1, 3).contiguous()
+        return cls(rows, cols, data.view(-1), scale.view(-1))
+
+    def to_ocp(self):
+        """(codes [rows, cols / 2], scale bytes [rows, cols / 32]) in row-major order."""
+        rb, kg = -(-self.rows // 32), -(-self.cols // 256)
+        c = self.data.view(rb, kg * 4, 2, 32, 16).permute(0, 3, 1, 2, 4).reshape(rb * 32, kg * 128)
+        s = self.scale.view(rb, kg, 2, 32, 4).permute(0, 3, 1, 4, 2).reshape(rb * 32, kg * 8)
+        return c[:self.rows, :self.cols // 2].contiguous(), s[:self.rows, :self.cols // 32].contiguous()
+
+    def dequantize(self, dtype=BF16, out=None):
+        """The values it stands for, [rows, cols] bf16 or fp32 (exact in both)."""
+        if out is None:
+            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.data.device)
+        return H.mxfp4_dequant(self, out)
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("mxfp4: inference only; call under torch.no_grad() or detach the inputs")
+
+
+def _rows2d(x):
+    """x [..., K] as [M, K] with unit column stride and rows on 16-byte boundaries (a copy where it has none)."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.stride(0) * x2.element_size()) % 16 or x2.data_ptr() % 16 \
+            or x2.stride(0) < x2.shape[1]:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def mxfp4_quantize(x, out=None):
+    """x [..., K] bf16 or fp32 (K a multiple of 32) -> MXFP4Matrix [M, K], M the product of the leading dimensions.
+    A block of 32 gets the scale 2^(floor(log2 max|x|) - 2), its values the nearest E2M1 number (ties to even,
+    saturated at 6); a block that holds an infinity or a NaN becomes NaN."""
+    if x.dtype not in (BF16, F32):
+        raise TypeError(f"mxfp4: expected bf16 or fp32, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise ValueError(f"mxfp4: the last dimension must be a positive multiple of 32, got {tuple(x.shape)}")
+    _no_grad(x)
+    x2 = _rows2d(x)
+    if out is None:
+        out = MXFP4Matrix.empty(x2.shape[0], x2.shape[1], x.device)
+    return H.mxfp4_quant(x2, out)
+
+
+def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, residual=None, gate=None):
+    """act(x @ weight.T + bias) with both operands in MXFP4 and fp32 accumulation; one rounding, of the stored value.
+    x: [..., K] bf16 or fp32 (quantised here), or an MXFP4Matrix; weight: MXFP4Matrix [N, K], N a multiple of 4;
+    bias bf16 [N]; gelu: tanh-GELU (bf16 output).  Returns [..., N] in out_dtype (bf16 or fp32), written to `out` if given.
+    residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned."""
+    if not isinstance(weight, MXFP4Matrix):
+        raise TypeError("mxfp4_linear: weight must be an MXFP4Matrix (mxfp4_quantize or MXFP4Matrix.from_ocp)")
+    packed = isinstance(x, MXFP4Matrix)
+    lead = (x.rows,) if packed else tuple(x.shape[:-1])
+    _no_grad(None if packed else x, bias, residual, gate)
+    N = weight.rows
+    if residual is not None:
+        if out is not None or gelu:
+            raise ValueError("mxfp4_linear: residual goes with neither out nor gelu")
+        out, epi = residual, H.EPI_RESID
+    else:
+        if gate is not None:
+            raise ValueError("mxfp4_linear: gate goes with residual")
+        if out is None:
+            out = torch.empty(lead + (N,), dtype=out_dtype, device=weight.device)
+        if gelu and out.dtype != BF16:
+            raise TypeError("mxfp4_linear: gelu writes bf16")
+        epi = H.EPI_BF16_GELU if gelu else (H.EPI_BF16 if out.dtype == BF16 else H.EPI_F32)
+    if tuple(out.shape) != lead + (N,):
+        raise ValueError(f"mxfp4_linear: expected an output of shape {lead + (N,)}, got {tuple(out.shape)}")
+    a = x if packed else mxfp4_quantize(x)
+    H.gemm_mxfp4(a, weight, out, bias, epi, gate)
+    return out
