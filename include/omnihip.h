@@ -327,6 +327,38 @@ int ovd_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out, int 
 int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
                    void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream);
 
+/* ---- Packed documents: tokens of several requests (videos, images, prompts of different sizes) in one row --------
+ *
+ * ovd_rope_positions: rotary embedding by explicit positions.  x, out [tokens, heads, head_dim] (bf16, or fp32 when
+ * x_is_f32; dense heads, token strides ldx / ldo; out may be x), pos [tokens, n_axes] int32 (fp32 when pos_is_f32).
+ * Pair p of a head turns by pos[t][axis[p]] * freq[p] REVOLUTIONS (freq double, axis int32, both [head_dim / 2] on the
+ * device; axis outside [0, n_axes): the pair passes through).  interleaved: pairs (2p, 2p + 1), else (p, p + head_dim/2);
+ * inverse: the opposite turn.  head_dim % 16 == 0, <= 512; n_axes <= 8.  Angles are 64-bit: positions may be large.
+ * The positions form of rope_apply (omnivideo/modules/model.py:37-65), which derives them from one grid per sample. */
+int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos, int pos_is_f32, int n_axes,
+                       const double* freq, const int32_t* axis, void* out, int64_t ldo, int64_t tokens, int heads,
+                       int head_dim, int interleaved, int inverse, void* stream);
+
+/* ovd_attn_packed_fwd_bf16: softmax attention inside documents.  q, out [total_q, q_heads, D], k, v [total_k, kv_heads, D]
+ * bf16 (dense heads, token strides *_ld), D = 64 or 128, q_heads a multiple of kv_heads (head h reads key head
+ * h / (q_heads / kv_heads)).  Document d: query rows [cu_q[d], cu_q[d+1]), key rows [cu_k[d], cu_k[d+1]) (device int32
+ * [docs + 1], ascending; values are clamped to the tensors).  Query i of a document with Lq queries and Lk keys sees
+ * its first Lk keys, with `causal` its first max(i + Lk - Lq + 1, prefix[d]) (prefix: device int32 [docs] or NULL).
+ * softcap > 0: scores s become softcap * tanh(s / softcap).  A query that sees no key gets zeros; rows outside every
+ * document are not written; keys and values outside a document do not enter it, whatever they hold.
+ * max_q / max_k: the longest document as the host knows it; they choose the launch (any value gives right results).
+ * workspace: with few query rows the keys are split over workgroups and joined, in
+ * ovd_attn_packed_workspace_bytes(...) (HOST) bytes, 16-byte aligned; NULL or smaller: not split.  It holds no state
+ * between calls; calls that may overlap need their own.
+ * The reference packs a padded batch this way for flash_attn_varlen_func (omnivideo/modules/attention.py:96-130). */
+int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int docs, int q_heads, int kv_heads, int head_dim, int64_t max_q,
+                                        int64_t max_k);
+int ovd_attn_packed_fwd_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int64_t total_q,
+                             int64_t total_k, const int32_t* cu_q, const int32_t* cu_k, int docs, int64_t max_q,
+                             int64_t max_k, int q_heads, int kv_heads, int head_dim, int64_t q_ld, int64_t k_ld,
+                             int64_t v_ld, int64_t o_ld, int causal, const int32_t* prefix, float softmax_scale,
+                             float softcap, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Source-video frames -> VAE encoder input, the device half of transform_frames_to_tensor
  * (tools/inference/generate_omni_v2v.py:306-343: CenterCrop, Resize on a PIL image = Pillow's 8-bit
  * bilinear resample, ToTensor, Normalize).  frames [T,H,W,3] uint8; the crop window (top, left,

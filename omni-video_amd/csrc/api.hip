@@ -46,6 +46,12 @@ int ovd_impl_mxfp4_quant(const void*, int, long, uint8_t*, uint8_t*, int, int, h
 int ovd_impl_mxfp4_dequant(const uint8_t*, const uint8_t*, void*, int, long, int, int, hipStream_t);
 int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
                         const float*, int, int, int, int, hipStream_t);
+int ovd_impl_rope_positions(const void*, int, long, const void*, int, int, const double*, const int*, void*, long, long,
+                            int, int, int, int, hipStream_t);
+long ovd_impl_attn_packed_workspace(long, int, int, int, int, long, long);
+int ovd_impl_attn_packed(const bf16_t*, const bf16_t*, const bf16_t*, bf16_t*, long, long, const int*, const int*, int, long,
+                         long, int, int, int, long, long, long, long, int, const int*, float, float, void*, long,
+                         hipStream_t);
 int ovd_impl_frames_resize(const uint8_t*, uint8_t*, float*, const int*, const int*, int, const int*, const int*, int,
                            const float*, long, int, int, int, int, int, int, int, int, hipStream_t);
 int ovd_impl_t5_attention(const bf16_t*, long, const bf16_t*, const int*, const int*, bf16_t*, long, int, int, int, int,
@@ -347,6 +353,31 @@ int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, c
                    void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream) {
     NONNULL(A); NONNULL(a_scale); NONNULL(W); NONNULL(w_scale); NONNULL(out);
     return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, ST(stream));
+}
+
+int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos, int pos_is_f32, int n_axes,
+                       const double* freq, const int32_t* axis, void* out, int64_t ldo, int64_t tokens, int heads,
+                       int head_dim, int interleaved, int inverse, void* stream) {
+    NONNULL(x); NONNULL(pos); NONNULL(freq); NONNULL(axis); NONNULL(out);
+    return ovd_impl_rope_positions(x, x_is_f32, ldx, pos, pos_is_f32, n_axes, freq, axis, out, ldo, tokens, heads,
+                                   head_dim, interleaved, inverse, ST(stream));
+}
+
+int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int docs, int q_heads, int kv_heads, int head_dim, int64_t max_q,
+                                        int64_t max_k) {
+    return ovd_impl_attn_packed_workspace(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k);
+}
+
+int ovd_attn_packed_fwd_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int64_t total_q,
+                             int64_t total_k, const int32_t* cu_q, const int32_t* cu_k, int docs, int64_t max_q,
+                             int64_t max_k, int q_heads, int kv_heads, int head_dim, int64_t q_ld, int64_t k_ld,
+                             int64_t v_ld, int64_t o_ld, int causal, const int32_t* prefix, float softmax_scale,
+                             float softcap, void* workspace, int64_t workspace_bytes, void* stream) {
+    NONNULL(q); NONNULL(out); NONNULL(cu_q); NONNULL(cu_k);
+    if (total_k > 0) { NONNULL(k); NONNULL(v); }
+    return ovd_impl_attn_packed(q, k, v, out, total_q, total_k, cu_q, cu_k, docs, max_q, max_k, q_heads, kv_heads, head_dim,
+                                q_ld, k_ld, v_ld, o_ld, causal, prefix, softmax_scale, softcap, workspace, workspace_bytes,
+                                ST(stream));
 }
 
 int ovd_resize_coeffs(int in_size, int out_size, int* bounds_host, int* coef_host, int ksize_cap) {

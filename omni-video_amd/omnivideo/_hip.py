@@ -52,6 +52,10 @@ SIGNATURES = {
     "ovd_mxfp4_quant": [_p, _i, _l, _p, _p, _i, _i, _p],
     "ovd_mxfp4_dequant": [_p, _p, _p, _i, _l, _i, _i, _p],
     "ovd_gemm_mxfp4": [_p, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _p],
+    "ovd_rope_positions": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _l, _l, _i, _i, _i, _i, _p],
+    "ovd_attn_packed_workspace_bytes": [_l, _i, _i, _i, _i, _l, _l],
+    "ovd_attn_packed_fwd_bf16": [_p, _p, _p, _p, _l, _l, _p, _p, _i, _l, _l, _i, _i, _i, _l, _l, _l, _l, _i, _p, _f, _f, _p,
+                                 _l, _p],
     "ovd_resize_coeffs": [_i, _i, _p, _p, _i],
     "ovd_frames_resize_normalize": [_p, _p, _p, _p, _p, _i, _p, _p, _i, _p, _l, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "ovd_t5_attention_bf16": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _i, _p],
@@ -77,7 +81,8 @@ SIGNATURES = {
     "ovd_peer_sum_f32": [_p, _p, _l, _i, _p],
 }
 
-SIZE_FUNCTIONS = ("ovd_flash_attn_workspace_bytes", "ovd_mxfp4_data_bytes", "ovd_mxfp4_scale_bytes")      # return int64
+SIZE_FUNCTIONS = ("ovd_flash_attn_workspace_bytes", "ovd_mxfp4_data_bytes", "ovd_mxfp4_scale_bytes",
+                  "ovd_attn_packed_workspace_bytes")                       # host functions that return int64
 
 EPI_BF16, EPI_BF16_GELU, EPI_F32, EPI_RESID = 0, 1, 2, 3
 UNIPC_COEF_STRIDE = 16
@@ -758,6 +763,69 @@ def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
         _, _, ldo = _rows(out)
         _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), out.data_ptr(),
                  ldo if M > 1 else N, None if gate is None else gate.data_ptr(), M, N, K, epilogue)
+    return out
+
+
+# ---------------------------------------------------------------------------- packed documents
+
+def _packed_heads(name, t):
+    """token stride of [T, N, D] with dense heads"""
+    if t.dim() != 3 or t.shape[1] < 1 or (t.shape[2] > 1 and t.stride(2) != 1) \
+            or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{name}: tensors must be [tokens, heads, head_dim] with dense (heads, head_dim)")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def rope_positions(x, pos, freq, axis, out, interleaved=True, inverse=False):
+    """x, out [T, N, D] bf16 or fp32, pos [T, A] int32 or fp32, freq fp64 [D / 2] (revolutions), axis int32 [D / 2]."""
+    ldx, ldo = _packed_heads("rope", x), _packed_heads("rope", out)
+    T, N, D = x.shape
+    if out.shape != x.shape or out.dtype != x.dtype or x.dtype not in (BF16, F32):
+        raise ValueError("rope: x and out must be bf16 or fp32 tensors of one shape and type")
+    if pos.dim() != 2 or pos.shape[0] != T or pos.dtype not in (torch.int32, F32) or not pos.is_contiguous():
+        raise ValueError(f"rope: positions must be contiguous int32 or fp32 [{T}, axes], got {tuple(pos.shape)} {pos.dtype}")
+    if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.numel() != D // 2 or axis.numel() != D // 2 \
+            or not freq.is_contiguous() or not axis.is_contiguous():
+        raise ValueError(f"rope: the frequency table is not one of {D // 2} pairs")
+    dev = _one_device(x, pos, freq, axis, out)
+    if T:
+        _call_on(dev, "ovd_rope_positions", x.data_ptr(), int(x.dtype == F32), ldx, pos.data_ptr(), int(pos.dtype == F32),
+                 pos.shape[1], freq.data_ptr(), axis.data_ptr(), out.data_ptr(), ldo, T, N, D, int(interleaved),
+                 int(inverse))
+    return out
+
+
+def attn_packed_workspace_bytes(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k):
+    """Bytes with which attn_packed splits long documents over workgroups when there are few query rows (0: no use).
+    Depends on the current device's compute units."""
+    return int(lib().ovd_attn_packed_workspace_bytes(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k))
+
+
+def attn_packed(q, k, v, cu_q, cu_k, out, max_q, max_k, causal=False, prefix=None, softmax_scale=None, softcap=0.0,
+                workspace=None):
+    """q, out [Tq, Nq, D], k, v [Tk, Nk, D] bf16; cu_q, cu_k int32 [documents + 1], prefix int32 [documents] or None;
+    see the header."""
+    q_ld, k_ld, v_ld, o_ld = (_packed_heads("attention", t) for t in (q, k, v, out))
+    Tq, Nq, D = q.shape
+    Tk, Nk, _ = k.shape
+    if any(t.dtype != BF16 for t in (q, k, v, out)):
+        raise TypeError("attention: q, k, v and out must be bf16")
+    if k.shape != v.shape or k.shape[2] != D or out.shape != q.shape or Nq % Nk:
+        raise ValueError(f"attention: shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)} out{tuple(out.shape)}")
+    docs = cu_q.numel() - 1
+    for t, n in ((cu_q, docs + 1), (cu_k, docs + 1)) + (((prefix, docs),) if prefix is not None else ()):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or docs < 1 or not t.is_contiguous():
+            raise ValueError("attention: cu_q and cu_k must be int32 [documents + 1], prefix int32 [documents]")
+    scale = float(softmax_scale) if softmax_scale is not None else D ** -0.5
+    dev = _one_device(q, k, v, out, cu_q, cu_k, prefix, workspace)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("attention: workspace must be a contiguous device tensor")
+    if Tq:
+        _call_on(dev, "ovd_attn_packed_fwd_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), Tq, Tk,
+                 cu_q.data_ptr(), cu_k.data_ptr(), docs, int(max_q), int(max_k), Nq, Nk, D, q_ld, k_ld, v_ld, o_ld,
+                 int(causal), None if prefix is None else prefix.data_ptr(), scale, float(softcap),
+                 None if workspace is None else workspace.data_ptr(),
+                 0 if workspace is None else workspace.numel() * workspace.element_size())
     return out
 
 
