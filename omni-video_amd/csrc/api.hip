@@ -46,6 +46,9 @@ int ovd_impl_mxfp4_quant(const void*, int, long, uint8_t*, uint8_t*, int, int, h
 int ovd_impl_mxfp4_dequant(const uint8_t*, const uint8_t*, void*, int, long, int, int, hipStream_t);
 int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
                         const float*, int, int, int, int, hipStream_t);
+long ovd_impl_linear_mxfp4_workspace(int, int);
+int ovd_impl_linear_mxfp4(const void*, int, long, const uint8_t*, const uint8_t*, const bf16_t*, void*, long, const float*,
+                          void*, long, int, int, int, int, hipStream_t);
 int ovd_impl_rope_positions(const void*, int, long, const void*, int, int, const double*, const int*, void*, long, long,
                             int, int, int, int, hipStream_t);
 long ovd_impl_attn_packed_workspace(long, int, int, int, int, long, long);
@@ -353,6 +356,16 @@ int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, c
                    void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream) {
     NONNULL(A); NONNULL(a_scale); NONNULL(W); NONNULL(w_scale); NONNULL(out);
     return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, ST(stream));
+}
+
+int64_t ovd_linear_mxfp4_workspace_bytes(int M, int K) { return M <= 0 || K <= 0 ? 0 : ovd_impl_linear_mxfp4_workspace(M, K); }
+
+int ovd_linear_mxfp4(const void* x, int x_is_f32, int64_t ldx, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
+                     void* out, int64_t ldo, const float* gate, void* workspace, int64_t workspace_bytes, int M, int N, int K,
+                     int epilogue, void* stream) {
+    NONNULL(x); NONNULL(W); NONNULL(w_scale); NONNULL(out);
+    return ovd_impl_linear_mxfp4(x, x_is_f32, ldx, W, w_scale, bias, out, ldo, gate, workspace, workspace_bytes, M, N, K,
+                                 epilogue, ST(stream));
 }
 
 int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos, int pos_is_f32, int n_axes,

@@ -300,6 +300,334 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
     }
 }
 
+// A handful of rows (M <= FEW_ROWS) straight from bf16 / fp32: every workgroup quantises all of x into LDS (a few thousand
+// values) under its first weight loads, so a token's layer is one launch.  A workgroup owns one block of 32 weight rows;
+// its waves take the k-groups in turn and meet as above.  LDS: codes [group][ks][h][FEW_ROWS][16], scales
+// [group][h][FEW_ROWS][4], then the partial sums.
+constexpr int FEW_ROWS = 8;
+constexpr int FEW_GRP = 8 * FEW_ROWS * 16 + 2 * FEW_ROWS * 4;       // LDS bytes per k-group
+constexpr int FEW_PART = 8 * 4 * 64 * 16;
+
+template <typename T, int EPI>
+__global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restrict__ x, long ldx, Operand W, Out o, int M, int K,
+                                                               int groups) {
+    extern __shared__ __attribute__((aligned(16))) char few_smem[];
+    char* codes = few_smem;
+    char* scales = few_smem + groups * (8 * FEW_ROWS * 16);
+    float4* part = reinterpret_cast<float4*>(few_smem + (groups * FEW_GRP + 15) / 16 * 16);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 31, h = lane >> 5;
+    Group w;
+    if (wave < groups) w = load_group(W, blockIdx.x, wave, groups, lane);
+    const int chunks = groups * 32;                       // 8-value chunks per row; a block's four sit in adjacent lanes
+    for (int i = tid; i < M * chunks; i += 512) {
+        const int m = i / chunks, c = i - m * chunks;
+        float v[8];
+        if (c * 8 < K) load8<T>(x + m * ldx + c * 8, v);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        uint32_t mx = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = umax(mx, __float_as_uint(v[j]) & 0x7fffffffu);
+        mx = umax(mx, __shfl_xor(mx, 1, 64));
+        mx = umax(mx, __shfl_xor(mx, 2, 64));
+        const uint32_t s = scale_byte(mx);
+        const float inv = inv_scale(s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        const int kg = c >> 5, ks = (c >> 3) & 3, hh = (c >> 2) & 1;
+        *reinterpret_cast<uint32_t*>(codes + ((kg * 4 + ks) * 2 + hh) * (FEW_ROWS * 16) + m * 16 + (c & 3) * 4) = pack_fp4x8(v);
+        if ((c & 3) == 0) scales[((kg * 2 + hh) * FEW_ROWS + m) * 4 + ks] = (char)s;
+    }
+    __syncthreads();
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    for (int kg = wave; kg < groups; kg += 8) {
+        Group a;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+            a.f[ks] = r < M ? *reinterpret_cast<const uint4*>(codes + ((kg * 4 + ks) * 2 + h) * (FEW_ROWS * 16) + r * 16)
+                            : make_uint4(0, 0, 0, 0);
+        a.s = r < M ? *reinterpret_cast<const int*>(scales + ((kg * 2 + h) * FEW_ROWS + r) * 4) : 0;
+        const Group wn = load_group(W, blockIdx.x, kg + 8 < groups ? kg + 8 : kg, groups, lane);
+        mfma_group(acc, w, a);
+        w = wn;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) part[(wave * 4 + g) * 64 + lane] = make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
+    __syncthreads();
+    if (wave >= 4) return;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float4 p = part[(k * 4 + wave) * 64 + lane];
+        y[0] += p.x;
+        y[1] += p.y;
+        y[2] += p.z;
+        y[3] += p.w;
+    }
+    const int n = blockIdx.x * 32 + 8 * wave + 4 * h;
+    if (r < M && n < W.rows) store4<EPI>(o, r, n, y);
+}
+
+// ------------------------------------------------------------------------------------------ product, many rows
+// The four-phase schedule of gemm256.hip on 256 x 256 output tiles: K-tiles of one k-group (128 bytes of codes per row,
+// 64 KiB for both operands), two LDS buffers, one 16 KiB half-tile staged per phase, DMA never drained inside the loop,
+// the two wave groups one barrier apart.  A phase is 8 v_mfma_scale_f32_32x32x64_f8f6f4 on fp4 operands: the matrix time
+// of the 4 e4m3 ones of fp8.hip's phase for twice the K, so LDS and DMA bytes per matrix cycle are the same.
+// The tile layout makes every DMA instruction 1 KiB of consecutive memory and every fragment read 1 KiB of consecutive
+// LDS: no swizzle.  Scales travel the same way, one 256-byte instruction per row block and K-tile (8 KiB of LDS for two
+// buffers); they are issued with phase 4, so any four consecutive phases hold 10 DMA instructions of a wave.
+constexpr int TM = 256, TN = 256;
+constexpr int PBUF = 2 * 8 * GRP_DATA;            // one buffer: A 8 row blocks x 4 KiB | W the same
+constexpr int SBUF = 2 * 8 * GRP_SCALE;           // its scales
+constexpr int BIG_LDS = 2 * PBUF + 2 * SBUF;
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// this wave's DMA sources: fragment `wave & 3` of two row blocks of either half, and the scales of row block `wave`
+struct Feed {
+    const uint8_t* data[4];      // instruction i of a tile: row block (i * 8 + wave) / 4, k-step wave & 3
+    const uint8_t* scale;
+};
+
+template <int HALF>
+__device__ __forceinline__ void stage_half(const Feed& f, long kg, char* part_wave) {
+    __builtin_amdgcn_global_load_lds(f.data[2 * HALF] + kg * GRP_DATA, (lds_ptr)(part_wave + (2 * HALF) * 8192), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(f.data[2 * HALF + 1] + kg * GRP_DATA, (lds_ptr)(part_wave + (2 * HALF + 1) * 8192), 16, 0, 0);
+}
+__device__ __forceinline__ void stage_scales(const Feed& fa, const Feed& fw, long kg, char* dst_wave) {
+    __builtin_amdgcn_global_load_lds(fa.scale + kg * GRP_SCALE, (lds_ptr)dst_wave, 4, 0, 0);
+    __builtin_amdgcn_global_load_lds(fw.scale + kg * GRP_SCALE, (lds_ptr)(dst_wave + 8 * GRP_SCALE), 4, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void phase_open() {
+    if (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (N == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+    if (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    if (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void phase_close() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+}
+
+struct Frag4 {
+    i32x4 k[4];                  // a row block's four k-steps
+};
+__device__ __forceinline__ i32x8 frag8(const i32x4& u) { return (i32x8){u[0], u[1], u[2], u[3], 0, 0, 0, 0}; }
+__device__ __forceinline__ Frag4 lds_frags(const char* p, int lane) {
+    Frag4 f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) f.k[ks] = *reinterpret_cast<const i32x4*>(p + ks * FRAG + lane * 16);
+    return f;
+}
+
+#define MX_STEP(KS)                                                                                                       \
+    a0 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.k[KS]), frag8(x[0].k[KS]), a0, 4, 4, KS, ws, KS, xs0);   \
+    a1 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.k[KS]), frag8(x[1].k[KS]), a1, 4, 4, KS, ws, KS, xs1);
+__device__ __forceinline__ void quadrant(f32x16& a0, f32x16& a1, const Frag4& w, int ws, const Frag4 (&x)[2], int xs0, int xs1) {
+    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+}
+#undef MX_STEP
+
+// TAIL 0: steady state, 1: next-to-last K-tile, 2: last
+template <int TAIL>
+__device__ __forceinline__ void k_tile(f32x16 (&acc)[2][4], char* smem, int buf, long kg1, long kg2, const Feed& fa, const Feed& fw,
+                                       int a_rd, int w_rd, int sa_rd, int sw_rd, int wave, int lane) {
+    const char* ca = smem + buf * PBUF + a_rd;
+    const char* cw = smem + buf * PBUF + PBUF / 2 + w_rd;
+    char* own = smem + buf * PBUF + wave * 1024;
+    char* oth = smem + (buf ^ 1) * PBUF + wave * 1024;
+    char* sbuf = smem + 2 * PBUF + buf * SBUF;
+    Frag4 w0, w1, af[2];
+    // phase 1
+    w0 = lds_frags(cw, lane);
+    af[0] = lds_frags(ca, lane);
+    af[1] = lds_frags(ca + GRP_DATA, lane);
+    int xs[4], ws[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        xs[i] = *reinterpret_cast<const int*>(sbuf + ((i >> 1) * 4 + (i & 1)) * GRP_SCALE + sa_rd);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ws[i] = *reinterpret_cast<const int*>(sbuf + (8 + i * 4) * GRP_SCALE + sw_rd);
+    if (TAIL < 2) stage_half<1>(fw, kg1, oth + PBUF / 2);
+    phase_open<TAIL == 2 ? 2 : 10>();
+    quadrant(acc[0][0], acc[0][1], w0, ws[0], af, xs[0], xs[1]);
+    phase_close();
+    // phase 2
+    w1 = lds_frags(cw + 4 * GRP_DATA, lane);
+    if (TAIL < 2) stage_half<1>(fa, kg1, oth);
+    phase_open<TAIL == 2 ? 0 : 10>();
+    quadrant(acc[1][0], acc[1][1], w1, ws[1], af, xs[0], xs[1]);
+    phase_close();
+    // phase 3
+    af[0] = lds_frags(ca + 4 * GRP_DATA, lane);
+    af[1] = lds_frags(ca + 5 * GRP_DATA, lane);
+    if (TAIL == 0) stage_half<0>(fw, kg2, own + PBUF / 2);
+    phase_open<-1>();
+    quadrant(acc[1][2], acc[1][3], w1, ws[1], af, xs[2], xs[3]);
+    phase_close();
+    // phase 4
+    if (TAIL == 0) {
+        stage_half<0>(fa, kg2, own);
+        stage_scales(fa, fw, kg2, sbuf + wave * GRP_SCALE);
+    }
+    phase_open<TAIL == 0 ? 10 : TAIL == 1 ? 4 : -1>();
+    quadrant(acc[0][2], acc[0][3], w0, ws[0], af, xs[2], xs[3]);
+    if (TAIL != 0) {
+        // a use in front of the closing barrier: the MFMAs of the last K-tiles would otherwise sink past it
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
+    }
+    phase_close();
+}
+
+template <int EPI>
+__device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, const Out& o, int groups, int tiles_m, int tiles_n,
+                                         int GM, int wide, int bid, char* smem) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));        // per-lane values are derived again for every tile instead of kept across the loop
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave >> 2, wc = wave & 3;
+    const int per_group = GM * tiles_n;
+    const int grp = bid / per_group, first_m = grp * GM;
+    const int gsz = min(tiles_m - first_m, GM);
+    const int tm = first_m + (bid % per_group) % gsz, tn = (bid % per_group) / gsz;
+    const long row0 = (long)tm * TM;
+    const int col0 = tn * TN;
+
+    Feed fa, fw;
+    {
+        const int a_last = (A.rows - 1) >> 5, w_last = (W.rows - 1) >> 5;      // row blocks past the last repeat it
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rb = (i * 8 + wave) >> 2, ks = wave & 3;
+            const long ra = min(tm * 8 + rb, a_last), rw = min(tn * 8 + rb, w_last);
+            fa.data[i] = A.data + ra * groups * GRP_DATA + ks * FRAG + lane * 16;
+            fw.data[i] = W.data + rw * groups * GRP_DATA + ks * FRAG + lane * 16;
+        }
+        fa.scale = A.scale + (long)min(tm * 8 + wave, a_last) * groups * GRP_SCALE + lane * 4;
+        fw.scale = W.scale + (long)min(tn * 8 + wave, w_last) * groups * GRP_SCALE + lane * 4;
+    }
+    const int a_rd = wr * 2 * GRP_DATA, w_rd = wc * GRP_DATA;
+    const int sa_rd = wr * 2 * GRP_SCALE + lane * 4, sw_rd = wc * GRP_SCALE + lane * 4;
+    f32x16 acc[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    char* const wd = smem + wave * 1024;
+    char* const sd = smem + 2 * PBUF + wave * GRP_SCALE;
+    stage_half<0>(fw, 0, wd + PBUF / 2);
+    stage_half<0>(fa, 0, wd);
+    stage_scales(fa, fw, 0, sd);
+    stage_half<1>(fw, 0, wd + PBUF / 2);
+    stage_half<1>(fa, 0, wd);
+    stage_half<0>(fw, 1, wd + PBUF + PBUF / 2);
+    stage_half<0>(fa, 1, wd + PBUF);
+    stage_scales(fa, fw, 1, sd + SBUF);
+    asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (wr == 1) __builtin_amdgcn_s_barrier();            // second half of the waves: one barrier behind
+    int t = 0;
+    for (; t + 2 < groups; ++t)
+        k_tile<0>(acc, smem, t & 1, t + 1, t + 2, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
+    k_tile<1>(acc, smem, t & 1, t + 1, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
+    ++t;
+    k_tile<2>(acc, smem, t & 1, 0, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
+    if (wr == 0) __builtin_amdgcn_s_barrier();            // balances the extra barrier above
+    asm volatile("" ::: "memory");
+
+    // acc[nh][mh * 2 + mb] register 4 g + j is out[m][n + j], m = row0 + mh * 128 + wr * 64 + mb * 32 + (lane & 31),
+    // n = col0 + nh * 128 + wc * 32 + 8 g + 4 (lane >> 5).  bf16 rows go through LDS (128 rows of 512 bytes per half,
+    // chunk c of row r at c ^ (r & 15)) so that 32 lanes store one 512-byte row segment.
+    constexpr bool NARROW = EPI == EPI_BF16 || EPI == EPI_BF16_GELU;
+    const int fr = lane & 31, fh = lane >> 5;
+    const bool staged = NARROW && wide;
+#pragma unroll
+    for (int mh = 0; mh < 2; ++mh) {
+        char* img = smem + mh * PBUF;
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+            const int rl = wr * 64 + mb * 32 + fr;
+            const long m = row0 + mh * 128 + rl;
+            if (!staged && m >= A.rows) continue;
+#pragma unroll
+            for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int nl = nh * 128 + wc * 32 + 8 * g + 4 * fh;
+                    const int n = col0 + nl;
+                    const f32x16& a16 = acc[nh][mh * 2 + mb];
+                    float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
+                    if (!staged) {
+                        if (n < W.rows) store4<EPI>(o, m, n, y);
+                        continue;
+                    }
+                    if (o.bias) {
+                        const uint2 b = *reinterpret_cast<const uint2*>(o.bias + min(n, W.rows - 4));
+                        y[0] += bf2f(b.x & 0xffff);
+                        y[1] += bf2f(b.x >> 16);
+                        y[2] += bf2f(b.y & 0xffff);
+                        y[3] += bf2f(b.y >> 16);
+                    }
+                    if constexpr (EPI == EPI_BF16_GELU) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = gelu_tanh_f(y[j]);
+                    }
+                    *reinterpret_cast<uint2*>(img + rl * 512 + (((nl >> 3) ^ (rl & 15)) << 4) + fh * 8) =
+                        make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
+                }
+        }
+        if (staged) {       // uniform: every thread reaches the barrier
+            __syncthreads();
+            const int rr = tid >> 5, cc = tid & 31;
+            const int n = col0 + cc * 8;
+            bf16_t* ob = reinterpret_cast<bf16_t*>(o.out) + n;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 16 + rr;
+                const long m = row0 + mh * 128 + r;
+                const uint4 v = *reinterpret_cast<const uint4*>(img + r * 512 + ((cc ^ (r & 15)) << 4));
+                if (m < A.rows) {
+                    if (n + 8 <= W.rows)
+                        __builtin_nontemporal_store((u32x4){v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(ob + m * o.ldo));
+                    else if (n < W.rows)
+                        *reinterpret_cast<uint2*>(ob + m * o.ldo) = make_uint2(v.x, v.y);
+                }
+            }
+        }
+    }
+}
+
+// Persistent, one workgroup per CU; the workgroups of an XCD take the tiles of that XCD's chunk of the walk in turn
+template <int EPI>
+__global__ void __launch_bounds__(512, 2) gemm_mxfp4_big_kernel(Operand A, Operand W, Out o, int groups, int tiles_m, int tiles_n,
+                                                                int GM, int wide) {
+    extern __shared__ __attribute__((aligned(16))) char big_smem[];
+    const int nwg = tiles_m * tiles_n;
+    const int xcd = blockIdx.x & 7, q = nwg >> 3, r = nwg & 7;
+    const int first = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
+    const int count = q + (xcd < r ? 1 : 0);
+    const int per_xcd = (gridDim.x + 7) >> 3;
+    for (int t = blockIdx.x >> 3; t < count; t += per_xcd) {
+        big_tile<EPI>(A, W, o, groups, tiles_m, tiles_n, GM, wide, first + t, big_smem);
+        __syncthreads();          // the LDS buffers are staged again by the next tile
+    }
+}
+
 }  // namespace
 
 static long mx_groups(long K) { return (K + KG - 1) / KG; }
@@ -344,9 +672,19 @@ int ovd_impl_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out,
     return 0;
 }
 
-int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uint8_t* w_data, const uint8_t* w_scale,
-                        const bf16_t* bias, void* out, long ldo, const float* gate, int M, int N, int K, int epilogue,
-                        hipStream_t st) {
+static bool few_rows(int M, int K) { return M <= FEW_ROWS && mx_groups(K) * FEW_GRP + FEW_PART + 16 <= 160 * 1024; }
+
+// bytes for the quantised x of ovd_impl_linear_mxfp4 (0: it needs none)
+long ovd_impl_linear_mxfp4_workspace(int M, int K) {
+    return few_rows(M, K) ? 0 : ovd_impl_mxfp4_data_bytes(M, K) + ovd_impl_mxfp4_scale_bytes(M, K);
+}
+
+int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
+                        const float*, int, int, int, int, hipStream_t);
+
+// the output side of both products
+static int check_out(int M, int N, int K, int epilogue, const void* out, long ldo, const void* bias, const void* gate,
+                     const void* w_data, const void* w_scale) {
     OVD_REQUIRE(M >= 0 && N > 0 && N % 4 == 0 && K > 0 && K % 32 == 0,
                 "gemm_mxfp4: M=%d N=%d K=%d not supported: N %% 4, K %% 32", M, N, K);
     OVD_REQUIRE(epilogue >= EPI_BF16 && epilogue <= EPI_RESID, "gemm_mxfp4: unknown epilogue %d", epilogue);
@@ -354,8 +692,52 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
     OVD_REQUIRE(ldo >= N && ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (epilogue <= EPI_BF16_GELU ? 8 : 16) == 0 &&
                     reinterpret_cast<uintptr_t>(bias) % 8 == 0 && reinterpret_cast<uintptr_t>(gate) % 16 == 0,
                 "gemm_mxfp4: out rows, bias and gate must be aligned to 4 values (ldo=%ld)", ldo);
-    OVD_REQUIRE(reinterpret_cast<uintptr_t>(a_data) % 16 == 0 && reinterpret_cast<uintptr_t>(w_data) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(a_scale) % 4 == 0 && reinterpret_cast<uintptr_t>(w_scale) % 4 == 0,
+    OVD_REQUIRE(reinterpret_cast<uintptr_t>(w_data) % 16 == 0 && reinterpret_cast<uintptr_t>(w_scale) % 4 == 0,
+                "gemm_mxfp4: operands must be 16-byte aligned");
+    return 0;
+}
+
+int ovd_impl_linear_mxfp4(const void* x, int x_is_f32, long ldx, const uint8_t* w_data, const uint8_t* w_scale,
+                          const bf16_t* bias, void* out, long ldo, const float* gate, void* workspace, long workspace_bytes,
+                          int M, int N, int K, int epilogue, hipStream_t st) {
+    if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
+    if (M == 0) return 0;
+    if (!few_rows(M, K)) {
+        const long nd = ovd_impl_mxfp4_data_bytes(M, K);
+        OVD_REQUIRE(workspace != nullptr && workspace_bytes >= ovd_impl_linear_mxfp4_workspace(M, K),
+                    "linear_mxfp4: %d rows of %d need %ld bytes of workspace, got %ld", M, K,
+                    ovd_impl_linear_mxfp4_workspace(M, K), workspace_bytes);
+        uint8_t* data = (uint8_t*)workspace;
+        if (ovd_impl_mxfp4_quant(x, x_is_f32, ldx, data, data + nd, M, K, st)) return 1;
+        return ovd_impl_gemm_mxfp4(data, data + nd, w_data, w_scale, bias, out, ldo, gate, M, N, K, epilogue, st);
+    }
+    OVD_REQUIRE(ldx >= K && ldx % (x_is_f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0,
+                "linear_mxfp4: rows must keep 16-byte alignment (ldx=%ld)", ldx);
+    const Operand W{w_data, w_scale, N};
+    const Out o{bias, out, ldo, gate};
+    const int groups = (int)mx_groups(K);
+    const size_t lds = (groups * FEW_GRP + 15) / 16 * 16 + FEW_PART;
+#define FEW(T, E)                                                                                                    \
+    {                                                                                                                \
+        static OvdLdsLimit lim;                                                                                      \
+        if (!lim.ensure(reinterpret_cast<const void*>(&linear_mxfp4_few_kernel<T, E>), lds))                         \
+            OVD_FAIL("linear_mxfp4: cannot reserve %zu bytes of LDS", lds);                                          \
+        hipLaunchKernelGGL((linear_mxfp4_few_kernel<T, E>), dim3(ceil_div(N, 32)), dim3(512), lds, st, (const T*)x, ldx, W, o, \
+                           M, K, groups);                                                                            \
+    }
+#define FEW_CASE(E) case E: if (x_is_f32) FEW(float, E) else FEW(bf16_t, E) break;
+    switch (epilogue) { FEW_CASE(EPI_BF16) FEW_CASE(EPI_BF16_GELU) FEW_CASE(EPI_F32) FEW_CASE(EPI_RESID) }
+#undef FEW_CASE
+#undef FEW
+    OVD_CHECK_LAUNCH("linear_mxfp4");
+    return 0;
+}
+
+int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uint8_t* w_data, const uint8_t* w_scale,
+                        const bf16_t* bias, void* out, long ldo, const float* gate, int M, int N, int K, int epilogue,
+                        hipStream_t st) {
+    if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
+    OVD_REQUIRE(reinterpret_cast<uintptr_t>(a_data) % 16 == 0 && reinterpret_cast<uintptr_t>(a_scale) % 4 == 0,
                 "gemm_mxfp4: operands must be 16-byte aligned");
     if (M == 0) return 0;
     const Operand A{a_data, a_scale, M}, W{w_data, w_scale, N};
@@ -372,9 +754,23 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
         hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(N, 32 * NT), ty), dim3(512),   \
                            lds, st, A, W, o, groups);                                                          \
     }
-#define GEMM_CASE(E) case E: if (M <= 32) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
+#define BIG(E)                                                                                                 \
+    {                                                                                                          \
+        static OvdLdsLimit lim;                                                                                \
+        if (!lim.ensure(reinterpret_cast<const void*>(&gemm_mxfp4_big_kernel<E>), BIG_LDS))                    \
+            OVD_FAIL("gemm_mxfp4: cannot reserve %d bytes of LDS", BIG_LDS);                                   \
+        hipLaunchKernelGGL((gemm_mxfp4_big_kernel<E>), dim3(min(tiles_m * tiles_n, cus)), dim3(512), BIG_LDS, st, A, W, o, \
+                           groups, tiles_m, tiles_n, 4, wide);                                                 \
+    }
+    const int tiles_m = ceil_div(M, TM), tiles_n = ceil_div(N, TN);
+    const int cus = max(8, ovd_device_cus() / 8 * 8);
+    OVD_REQUIRE((long)tiles_m * tiles_n < (1L << 30), "gemm_mxfp4: grid too large");
+    const bool big = groups >= 2 && (long)tiles_m * tiles_n >= cus / 2;
+    const int wide = (ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) ? 1 : 0;
+#define GEMM_CASE(E) case E: if (big) BIG(E) else if (M <= 32) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
     switch (epilogue) { GEMM_CASE(EPI_BF16) GEMM_CASE(EPI_BF16_GELU) GEMM_CASE(EPI_F32) GEMM_CASE(EPI_RESID) }
 #undef GEMM_CASE
+#undef BIG
 #undef DIRECT
     OVD_CHECK_LAUNCH("gemm_mxfp4");
     return 0;

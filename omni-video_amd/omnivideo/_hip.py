@@ -52,6 +52,8 @@ SIGNATURES = {
     "ovd_mxfp4_quant": [_p, _i, _l, _p, _p, _i, _i, _p],
     "ovd_mxfp4_dequant": [_p, _p, _p, _i, _l, _i, _i, _p],
     "ovd_gemm_mxfp4": [_p, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _p],
+    "ovd_linear_mxfp4_workspace_bytes": [_i, _i],
+    "ovd_linear_mxfp4": [_p, _i, _l, _p, _p, _p, _p, _l, _p, _p, _l, _i, _i, _i, _i, _p],
     "ovd_rope_positions": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _l, _l, _i, _i, _i, _i, _p],
     "ovd_attn_packed_workspace_bytes": [_l, _i, _i, _i, _i, _l, _l],
     "ovd_attn_packed_fwd_bf16": [_p, _p, _p, _p, _l, _l, _p, _p, _i, _l, _l, _i, _i, _i, _l, _l, _l, _l, _i, _p, _f, _f, _p,
@@ -82,7 +84,7 @@ SIGNATURES = {
 }
 
 SIZE_FUNCTIONS = ("ovd_flash_attn_workspace_bytes", "ovd_mxfp4_data_bytes", "ovd_mxfp4_scale_bytes",
-                  "ovd_attn_packed_workspace_bytes")                       # host functions that return int64
+                  "ovd_linear_mxfp4_workspace_bytes", "ovd_attn_packed_workspace_bytes")                       # host functions that return int64
 
 EPI_BF16, EPI_BF16_GELU, EPI_F32, EPI_RESID = 0, 1, 2, 3
 UNIPC_COEF_STRIDE = 16
@@ -684,52 +686,46 @@ def gemm_fp8(a8, w8, w_scale, out, bias=None, epilogue=EPI_BF16, a_scale=None, a
 
 # ---------------------------------------------------------------------------- MXFP4
 
-def _call_on(device, name, *args):
-    """_call with `device` current, on that device's current stream (appended as the last argument)."""
-    if device.index == torch.cuda.current_device():
-        _call(name, *args, _stream())
+def _call_on(index, name, *args):
+    """_call on the current stream (appended as the last argument) of device `index`, made current for the call."""
+    if index == torch.cuda.current_device():
+        _call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _call(name, *args, _stream())
+        with torch.cuda.device(index):
+            _call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _one_device(*tensors):
-    """The HIP device that all given tensors (None skipped) are on."""
+    """Index of the HIP device that all given tensors (None skipped) are on."""
     dev = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("libomnihip works on device tensors only (got a CPU tensor)")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"tensors are on different devices ({dev}, {t.device})")
-        dev = t.device
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise ValueError("libomnihip works on device tensors only (got a CPU tensor)")
+            if dev is not None:
+                raise ValueError(f"tensors are on different devices (cuda:{dev}, cuda:{d})")
+            dev = d
     return dev
 
 
 def mxfp4_bytes(rows, cols):
-    """(bytes of codes, bytes of scales) of an MXFP4 matrix [rows, cols]."""
+    """(bytes of codes, bytes of scales) of an MXFP4 matrix [rows, cols]: the header's layout."""
     if rows < 0 or cols <= 0 or cols % 32:
         raise ValueError(f"mxfp4: a [{rows}, {cols}] matrix has no blocks of 32")
-    L = lib()
-    return int(L.ovd_mxfp4_data_bytes(rows, cols)), int(L.ovd_mxfp4_scale_bytes(rows, cols))
-
-
-def _mx_operand(m):
-    nd, ns = mxfp4_bytes(m.rows, m.cols)
-    for t, n in ((m.data, nd), (m.scale, ns)):
-        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < n:
-            raise ValueError(f"mxfp4: the buffers do not hold a [{m.rows}, {m.cols}] matrix")
-    return m.data.data_ptr(), m.scale.data_ptr()
+    groups = -(-rows // 32) * -(-cols // 256)
+    return 4096 * groups, 256 * groups
 
 
 def mxfp4_quant(x, m):
     """x bf16 / fp32 [M, K] (rows 16-byte aligned) -> m (MXFP4 matrix of that shape)."""
     M, K = x.shape
-    if (m.rows, m.cols) != (M, K) or x.dtype not in (BF16, F32) or (K > 1 and x.stride(1) != 1):
+    if m.rows != M or m.cols != K or x.dtype not in (BF16, F32) or (K > 1 and x.stride(1) != 1):
         raise ValueError("mxfp4: needs bf16 or fp32 rows of the matrix's shape")
-    dev = _one_device(x, m.data, m.scale)
-    d, s = _mx_operand(m)
+    dev = _one_device(x, m.buf)
+    d, s = m.pointers()
     if M:
         _call_on(dev, "ovd_mxfp4_quant", x.data_ptr(), int(x.dtype == F32), x.stride(0) if M > 1 else K, d, s, M, K)
     return m
@@ -738,31 +734,73 @@ def mxfp4_quant(x, m):
 def mxfp4_dequant(m, out):
     if tuple(out.shape) != (m.rows, m.cols) or out.dtype not in (BF16, F32) or (m.cols > 1 and out.stride(1) != 1):
         raise ValueError("mxfp4: out must be bf16 or fp32 rows of the matrix's shape")
-    dev = _one_device(out, m.data, m.scale)
-    d, s = _mx_operand(m)
+    dev = _one_device(out, m.buf)
+    d, s = m.pointers()
     if m.rows:
         _call_on(dev, "ovd_mxfp4_dequant", d, s, out.data_ptr(), int(out.dtype == F32),
                  out.stride(0) if m.rows > 1 else m.cols, m.rows, m.cols)
     return out
 
 
-def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
-    """out = epilogue(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; out [..., N] with a uniform row stride."""
-    M, N, K = a.rows, w.rows, a.cols
-    if w.cols != K or out.numel() != M * N or out.shape[-1] != N:
-        raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}] out{tuple(out.shape)}")
+def _row_stride(name, t, N):
+    """row stride of [..., N] whose leading dimensions collapse to uniformly spaced rows"""
+    if t.is_contiguous():
+        return N
+    M, C, ld = _rows(t)
+    if C != N:
+        raise ValueError(f"{name}: rows of {C}, expected {N}")
+    return ld if M > 1 else N
+
+
+def _mx_out(name, out, M, N, bias, epilogue, gate):
+    """checks of a product's output side; returns its row stride"""
+    if out.numel() != M * N or out.shape[-1] != N:
+        raise ValueError(f"{name}: expected [{M}, {N}] outputs, got {tuple(out.shape)}")
     want = BF16 if epilogue in (EPI_BF16, EPI_BF16_GELU) else F32
     for v, dt in ((bias, BF16), (gate, F32)):
         if v is not None and (v.numel() != N or not v.is_contiguous() or v.dtype != dt):
-            raise ValueError(f"gemm_mxfp4: bias (bf16) and gate (fp32) must be contiguous rows of length {N}")
+            raise ValueError(f"{name}: bias (bf16) and gate (fp32) must be contiguous rows of length {N}")
     if out.dtype != want:
-        raise TypeError(f"gemm_mxfp4: this epilogue writes {want}, out is {out.dtype}")
-    dev = _one_device(a.data, a.scale, w.data, w.scale, out, bias, gate)
-    (ad, asc), (wd, wsc) = _mx_operand(a), _mx_operand(w)
+        raise TypeError(f"{name}: this epilogue writes {want}, out is {out.dtype}")
+    return _row_stride(name, out, N)
+
+
+def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
+    """out = epilogue(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; out [..., N] with a uniform row stride."""
+    M, N, K = a.rows, w.rows, a.cols
+    if w.cols != K:
+        raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}]")
+    ldo = _mx_out("gemm_mxfp4", out, M, N, bias, epilogue, gate)
+    dev = _one_device(a.buf, w.buf, out, bias, gate)
+    (ad, asc), (wd, wsc) = a.pointers(), w.pointers()
     if M:
-        _, _, ldo = _rows(out)
         _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), out.data_ptr(),
-                 ldo if M > 1 else N, None if gate is None else gate.data_ptr(), M, N, K, epilogue)
+                 ldo, None if gate is None else gate.data_ptr(), M, N, K, epilogue)
+    return out
+
+
+MXFP4_FEW_ROWS = 8           # up to this many rows linear_mxfp4 quantises inside the product (one launch)
+
+
+def linear_mxfp4(x, w, out, bias=None, epilogue=EPI_BF16, gate=None):
+    """out = epilogue(quantised x @ w.T + bias), x bf16 / fp32 [M, K] with 16-byte aligned rows."""
+    M, K = x.shape
+    N = w.rows
+    if w.cols != K or x.dtype not in (BF16, F32) or x.stride(1) != 1:
+        raise ValueError(f"linear_mxfp4: shape mismatch x[{M},{K}] {x.dtype} w[{N},{w.cols}]")
+    ldo = _mx_out("linear_mxfp4", out, M, N, bias, epilogue, gate)
+    dev = _one_device(x, w.buf, out, bias, gate)
+    if not M:
+        return out
+    ws, ws_ptr, nb = None, None, 0
+    if M > MXFP4_FEW_ROWS or K > 16384:
+        nb = int(lib().ovd_linear_mxfp4_workspace_bytes(M, K))
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+        ws_ptr = ws.data_ptr()
+    wd, wsc = w.pointers()
+    _call_on(dev, "ovd_linear_mxfp4", x.data_ptr(), int(x.dtype == F32), x.stride(0) if M > 1 else K, wd, wsc,
+             None if bias is None else bias.data_ptr(), out.data_ptr(), ldo, None if gate is None else gate.data_ptr(),
+             ws_ptr, nb, M, N, K, epilogue)
     return out
 
 

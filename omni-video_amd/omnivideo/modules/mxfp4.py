@@ -15,8 +15,35 @@ class MXFP4Matrix:
     """A [rows, cols] matrix in MXFP4, its codes and scales in the order in which the matrix instructions read them
     (include/omnihip.h).  Made by `mxfp4_quantize` or `from_ocp`; a layer's weights are laid out once."""
 
-    def __init__(self, rows, cols, data, scale):
-        self.rows, self.cols, self.data, self.scale = rows, cols, data, scale
+    __slots__ = ("rows", "cols", "buf", "_data_bytes")
+
+    def __init__(self, rows, cols, buf):
+        """buf: uint8 device buffer, the codes followed by the scales (H.mxfp4_bytes of each)."""
+        nd, ns = H.mxfp4_bytes(rows, cols)
+        if buf.dtype != U8 or buf.dim() != 1 or not buf.is_contiguous() or buf.numel() != nd + ns or buf.data_ptr() % 16:
+            raise ValueError(f"mxfp4: the buffer does not hold a [{rows}, {cols}] matrix ({nd} + {ns} bytes)")
+        self.rows, self.cols, self.buf, self._data_bytes = rows, cols, buf, nd
+
+    @classmethod
+    def empty(cls, rows, cols, device):
+        """Uninitialised storage for a [rows, cols] matrix (cols a multiple of 32)."""
+        nd, ns = H.mxfp4_bytes(rows, cols)
+        m = cls.__new__(cls)
+        m.rows, m.cols, m.buf, m._data_bytes = rows, cols, torch.empty(nd + ns, dtype=U8, device=device), nd
+        return m
+
+    def pointers(self):
+        """Device addresses of the codes and the scales."""
+        p = self.buf.data_ptr()
+        return p, p + self._data_bytes
+
+    @property
+    def data(self):
+        return self.buf[:self._data_bytes]
+
+    @property
+    def scale(self):
+        return self.buf[self._data_bytes:]
 
     @property
     def shape(self):
@@ -24,13 +51,7 @@ class MXFP4Matrix:
 
     @property
     def device(self):
-        return self.data.device
-
-    @classmethod
-    def empty(cls, rows, cols, device):
-        """Uninitialised storage for a [rows, cols] matrix (cols a multiple of 32)."""
-        nd, ns = H.mxfp4_bytes(rows, cols)
-        return cls(rows, cols, torch.empty(nd, dtype=U8, device=device), torch.empty(ns, dtype=U8, device=device))
+        return self.buf.device
 
     @classmethod
     def from_ocp(cls, codes, scales):
@@ -52,7 +73,7 @@ class MXFP4Matrix:
         # [rb, r, kt, h, 16 bytes] -> [rb, kt, h, r, 16];  [rb, r, kg, ks, h] -> [rb, kg, h, r, ks]
         data = c.view(rb, 32, kg * 4, 2, 16).permute(0, 2, 3, 1, 4).contiguous()
         scale = s.view(rb, 32, kg, 4, 2).permute(0, 2, 4, 1, 3).contiguous()
-        return cls(rows, cols, data.view(-1), scale.view(-1))
+        return cls(rows, cols, torch.cat((data.view(-1), scale.view(-1))))
 
     def to_ocp(self):
         """(codes [rows, cols / 2], scale bytes [rows, cols / 32]) in row-major order."""
@@ -64,32 +85,37 @@ class MXFP4Matrix:
     def dequantize(self, dtype=BF16, out=None):
         """The values it stands for, [rows, cols] bf16 or fp32 (exact in both)."""
         if out is None:
-            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.data.device)
+            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.buf.device)
         return H.mxfp4_dequant(self, out)
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError("mxfp4: inference only; call under torch.no_grad() or detach the inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("mxfp4: inference only; call under torch.no_grad() or detach the inputs")
 
 
 def _rows2d(x):
     """x [..., K] as [M, K] with unit column stride and rows on 16-byte boundaries (a copy where it has none)."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.stride(0) * x2.element_size()) % 16 or x2.data_ptr() % 16 \
-            or x2.stride(0) < x2.shape[1]:
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    ld = x2.stride(0)
+    if x2.stride(1) != 1 or ld < x2.shape[1] or (ld * x2.element_size()) % 16 or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
+
+
+def _check_input(x):
+    if x.dtype not in (BF16, F32):
+        raise TypeError(f"mxfp4: expected bf16 or fp32, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise ValueError(f"mxfp4: the last dimension must be a positive multiple of 32, got {tuple(x.shape)}")
 
 
 def mxfp4_quantize(x, out=None):
     """x [..., K] bf16 or fp32 (K a multiple of 32) -> MXFP4Matrix [M, K], M the product of the leading dimensions.
     A block of 32 gets the scale 2^(floor(log2 max|x|) - 2), its values the nearest E2M1 number (ties to even,
     saturated at 6); a block that holds an infinity or a NaN becomes NaN."""
-    if x.dtype not in (BF16, F32):
-        raise TypeError(f"mxfp4: expected bf16 or fp32, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 32:
-        raise ValueError(f"mxfp4: the last dimension must be a positive multiple of 32, got {tuple(x.shape)}")
+    _check_input(x)
     _no_grad(x)
     x2 = _rows2d(x)
     if out is None:
@@ -105,7 +131,9 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
     if not isinstance(weight, MXFP4Matrix):
         raise TypeError("mxfp4_linear: weight must be an MXFP4Matrix (mxfp4_quantize or MXFP4Matrix.from_ocp)")
     packed = isinstance(x, MXFP4Matrix)
-    lead = (x.rows,) if packed else tuple(x.shape[:-1])
+    if not packed:
+        _check_input(x)
+    lead = (x.rows,) if packed else x.shape[:-1]
     _no_grad(None if packed else x, bias, residual, gate)
     N = weight.rows
     if residual is not None:
@@ -116,12 +144,12 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
         if gate is not None:
             raise ValueError("mxfp4_linear: gate goes with residual")
         if out is None:
-            out = torch.empty(lead + (N,), dtype=out_dtype, device=weight.device)
+            out = torch.empty((*lead, N), dtype=out_dtype, device=weight.buf.device)
         if gelu and out.dtype != BF16:
             raise TypeError("mxfp4_linear: gelu writes bf16")
         epi = H.EPI_BF16_GELU if gelu else (H.EPI_BF16 if out.dtype == BF16 else H.EPI_F32)
-    if tuple(out.shape) != lead + (N,):
-        raise ValueError(f"mxfp4_linear: expected an output of shape {lead + (N,)}, got {tuple(out.shape)}")
-    a = x if packed else mxfp4_quantize(x)
-    H.gemm_mxfp4(a, weight, out, bias, epi, gate)
-    return out
+    if out.shape != (*lead, N):
+        raise ValueError(f"mxfp4_linear: expected an output of shape {(*lead, N)}, got {tuple(out.shape)}")
+    if packed:
+        return H.gemm_mxfp4(x, weight, out, bias, epi, gate)
+    return H.linear_mxfp4(_rows2d(x), weight, out, bias, epi, gate)

@@ -122,7 +122,8 @@ def test_ocp_round_trip(X):
 
 
 SHAPES = [(1, 4, 32), (1, 5120, 5120), (2, 36, 288), (17, 260, 96), (31, 128, 1024), (32, 1536, 256), (33, 64, 2336),
-          (64, 512, 320), (130, 100, 512), (550, 1536, 8960), (700, 772, 4096), (2049, 512, 1536), (1300, 1280, 96)]
+          (64, 512, 320), (130, 100, 512), (550, 1536, 8960), (700, 772, 4096), (2049, 512, 1536), (1300, 1280, 96),
+          (8000, 1100, 512), (3333, 2564, 1056), (4127, 2052, 288)]
 
 
 def close(got, want, bound, dtype):
@@ -166,7 +167,8 @@ def test_linear_epilogues(X, M, N, K):
 def test_linear_exact_on_small_integers(X):
     """whole numbers with scale 1 have exact sums: a wrong lane, block order, nibble order or scale byte shows as a
     wrong whole number.  Blocks get different scales, so each scale has to meet its own block."""
-    for M, N, K in ((40, 68, 608), (1, 132, 1056), (300, 512, 256), (1030, 1536, 768)):
+    for M, N, K in ((40, 68, 608), (1, 132, 1056), (300, 512, 256), (1030, 1536, 768), (5000, 1668, 1312),
+                    (16000, 516, 512)):
         g = torch.Generator().manual_seed(M)
         lut = torch.tensor([0.0, 1.0, 2.0, 3.0, 4.0, 6.0])
         a = lut[torch.randint(0, 6, (M, K), generator=g)] * (torch.randint(0, 2, (M, K), generator=g) * 2 - 1)
@@ -187,11 +189,30 @@ def test_linear_quantises_its_input(X):
     assert torch.equal(y.view(150, 256), X.mxfp4_linear(X.mxfp4_quantize(x), w))
     assert torch.equal(X.mxfp4_linear(x.float(), w), y)
     assert X.mxfp4_linear(x[:0], w).shape == (0, 50, 256)
-    for rows in (1, 7, 32, 33):                                # few rows: the same sums as among many
-        assert torch.equal(X.mxfp4_linear(x[0, :rows], w, out_dtype=F32), X.mxfp4_linear(X.mxfp4_quantize(x[0, :rows]), w, out_dtype=F32))
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 64, 512), (300, 1536, 256), (1500, 1280, 512)])
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 33])
+@pytest.mark.parametrize("K,N", [(32, 4), (512, 256), (1120, 100), (13824, 64), (17408, 36), (30720, 32)])
+def test_linear_of_few_rows_equals_quantise_then_product(X, M, K, N):
+    """one launch or several: the same codes, and the same order of sums up to 32 rows"""
+    w = X.mxfp4_quantize(randn((N, K), 1, 1 / math.sqrt(K)).cuda())
+    bias, gate = randn((N,), 4).to(BF16).cuda(), randn((N,), 5).cuda()
+    for dt in (BF16, F32):
+        x = randn((M, K + 32), K, 3.0).to(dt).cuda()[:, 32:]
+        x[0, :40] = 0
+        a = X.mxfp4_quantize(x)
+        for kw in (dict(), dict(out_dtype=F32), dict(gelu=True)):
+            assert torch.equal(X.mxfp4_linear(x, w, bias, **kw), X.mxfp4_linear(a, w, bias, **kw))
+        r0 = randn((M, N), 6).cuda()
+        assert torch.equal(X.mxfp4_linear(x, w, residual=r0.clone(), gate=gate), X.mxfp4_linear(a, w, residual=r0.clone(), gate=gate))
+        A, W = a.dequantize(F32).double(), w.dequantize(F32).double()
+        close(X.mxfp4_linear(x, w, out_dtype=F32), A @ W.t(), K * 2.0 ** -23 * (A.abs() @ W.abs().t()), F32)
+    x[0, 5] = math.inf
+    y = X.mxfp4_linear(x, w)
+    assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 64, 512), (300, 1536, 256), (1500, 1280, 512), (4100, 2052, 512)])
 def test_linear_writes_only_its_rows(X, M, N, K):
     a, w, _, _ = operands(X, M, N, K, 9)
     for dt in (BF16, F32):

@@ -36,6 +36,9 @@ def test_sizes():
     assert H.mxfp4_bytes(1, 32) == (4096, 256)
     assert H.mxfp4_bytes(33, 257 * 32) == (2 * 33 * 4096, 2 * 33 * 256)
     assert H.mxfp4_bytes(0, 64) == (0, 0)
+    L = H.lib()
+    for rows, cols in ((1, 32), (31, 256), (32, 288), (33, 13824), (40560, 8960)):
+        assert H.mxfp4_bytes(rows, cols) == (L.ovd_mxfp4_data_bytes(rows, cols), L.ovd_mxfp4_scale_bytes(rows, cols))
     for bad in ((1, 0), (1, 48), (-1, 32)):
         with pytest.raises(ValueError):
             H.mxfp4_bytes(*bad)
@@ -83,9 +86,10 @@ def test_python_entries_refuse():
         mxfp4_linear(a, w, out=torch.zeros(4, 9))
     with pytest.raises(ValueError, match="length"):
         mxfp4_linear(a, w, bias=torch.zeros(7, dtype=torch.bfloat16))
-    short = MXFP4Matrix(8, 64, w.data[:16], w.scale)
-    with pytest.raises(ValueError, match="do not hold"):
-        H._mx_operand(short)
+    for buf in (w.buf[:-1], w.buf.view(torch.int8), w.buf.view(2, -1)):
+        with pytest.raises(ValueError, match="does not hold"):
+            MXFP4Matrix(8, 64, buf)
+    assert MXFP4Matrix(8, 64, w.buf).to_ocp()[0].shape == (8, 32)
 
 
 def test_c_entries_refuse_before_any_launch():
@@ -108,6 +112,11 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, p, 1, 8, 32, 0, None, why=b"gate")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 4, None, 1, 8, 32, 0, None, why=b"ldo")
     refused("ovd_gemm_mxfp4", p, p, p + 8, p, None, p, 8, None, 1, 8, 32, 0, None, why=b"16-byte")
+    refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, None, 0, 9, 8, 32, 0, None, why=b"workspace")
+    refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, p, 4351, 9, 8, 32, 0, None, why=b"workspace")
+    refused("ovd_linear_mxfp4", p, 0, 33, p, p, None, p, 8, None, None, 0, 2, 8, 32, 0, None, why=b"alignment")
+    refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, None, 0, 2, 8, 32, 5, None, why=b"epilogue")
+    assert L.ovd_linear_mxfp4_workspace_bytes(8, 13824) == 0 and L.ovd_linear_mxfp4_workspace_bytes(9, 32) == 4352
     assert L.ovd_gemm_mxfp4(p, p, p, p, None, p, 8, None, 0, 8, 32, 0, None) == 0        # no rows: nothing to do
 
 
