@@ -27,6 +27,7 @@ namespace {
 
 constexpr int BKV = 64;                       // keys per tile
 constexpr float NEG_INF = -__builtin_inff();
+constexpr float RESCALE_THR = 6.0f;
 
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
 typedef __attribute__((address_space(3))) bf16x4_t* lds_b4_ptr;
@@ -72,10 +73,9 @@ __device__ __forceinline__ void doc_range(const Args& a, int d, int& q0, int& lq
     lk = min(max(a.cu_k[d + 1], k0), a.total_k) - k0;
 }
 
-// document and row block (of ROWS rows) of work item `blk`, and how many items follow it; false past the last one
+// document and row block (of ROWS rows) of work item `blk`; false past the last one
 template <int ROWS>
-__device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int& doc, int& rb, int& left) {
-    bool found = false;
+__device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int& doc, int& rb) {
     for (int d0 = 0; d0 < a.docs; d0 += 64) {
         const int d = d0 + lane;
         int n = 0;
@@ -90,22 +90,17 @@ __device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int
             const int up = __shfl_up(incl, s, 64);
             if (lane >= s) incl += up;
         }
-        const int sum = __shfl(incl, 63, 64);
-        if (found) {
-            left += sum;
-            continue;
-        }
         const unsigned long long hit = __ballot(blk < incl);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             doc = d0 + l;
             rb = blk - __shfl(incl - n, l, 64);
-            left = sum - blk - 1;
-            found = true;
+            if (a.causal) rb = __shfl(n, l, 64) - 1 - rb;          // the longest rows first
+            return true;
         }
-        blk -= sum;
+        blk -= __shfl(incl, 63, 64);
     }
-    return found;
+    return false;
 }
 
 __device__ __forceinline__ int visible(const Args& a, int i, int lq, int lk, int prefix) {
@@ -126,11 +121,289 @@ __device__ __forceinline__ float* ws_stat(const Args& a, int split, long row) {
     return a.ws + a.n_splits * rows * D + (split * rows + row) * 2;
 }
 
+// DMA of one operand: 64-row tiles HBM -> LDS.  A wave's instruction covers RPI rows; rows past the document's last key
+// repeat it.  Tile bases advance in 64 bits, offsets inside a tile are 32 bits.
+template <int D, int NW, bool IS_K>
+struct Stream {
+    static constexpr int CPR = D / 8, RPI = 64 / CPR, N = BKV / RPI / NW;
+    const char* base;        // first key row of the document, this head
+    long ld2;                // bytes between rows
+    int lk;                  // keys of the document
+    unsigned off[NW == 1 ? 1 : N];       // this lane's offsets in a whole tile
+    __device__ __forceinline__ unsigned offset(int i, int lim, int wave, int lane) const {
+        const int r = (i * NW + wave) * RPI + lane / CPR, c = lane % CPR;
+        const int cs = IS_K ? (D == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) : (D == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2));
+        return (unsigned)min(r, lim) * (unsigned)ld2 + (unsigned)cs * 16u;
+    }
+    __device__ __forceinline__ void init(const bf16_t* first, long ld, int keys, int wave, int lane) {
+        base = reinterpret_cast<const char*>(first);
+        ld2 = ld * 2;
+        lk = keys;
+        if constexpr (NW > 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) off[i] = offset(i, BKV, wave, lane);
+        }
+    }
+    __device__ __forceinline__ void stage(int t, char* dst, int wave, int lane) const {
+        const char* tb = base + (long)t * BKV * ld2;
+        const int lim = lk - 1 - t * BKV;
+        if (NW > 1 && lim >= BKV - 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                __builtin_amdgcn_global_load_lds(tb + off[NW > 1 ? i : 0], (lds_ptr)(dst + (i * NW + wave) * 1024), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                __builtin_amdgcn_global_load_lds(tb + offset(i, lim, wave, lane), (lds_ptr)(dst + (i * NW + wave) * 1024), 16, 0, 0);
+        }
+    }
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
+
+template <int D>
+__device__ __forceinline__ bf16x8 read_v(const char* sv, int st, int db, int lane) {
+    const int g = lane >> 4, i16 = lane & 15, qd = i16 >> 2, pp = i16 & 3;
+    const int kr = 16 * st + 4 * (g >> 1) + qd;
+    const int ch = db * 4 + 2 * (g & 1) + (pp >> 1);
+    const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4_ptr)(sv + v_off<D>(kr, ch) + 8 * (pp & 1)));
+    const bf16x4_t h4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4_ptr)(sv + v_off<D>(kr + 8, ch) + 8 * (pp & 1)));
+    const uint2 lo2 = __builtin_bit_cast(uint2, lo), hi2 = __builtin_bit_cast(uint2, h4);
+    return __builtin_bit_cast(bf16x8, make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
+}
+
+// scores of a capped tile in units of log2: cap log2(e) tanh(s scale / cap), tanh(x) = 1 - 2 / (1 + e^2x) (both ends
+// saturate without overflow)
+__device__ __forceinline__ void cap_scores(f32x16& s, float cap_in, float cap_out) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        s[j] = __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * cap_in)), cap_out);
+}
+
+__device__ __forceinline__ void mask_scores(f32x16& s0, f32x16& s1, int key0, int nvis, int hi) {
+    const int left = nvis - key0 - 4 * hi;              // this lane's keys sit at (r & 3) + 8 (r >> 2) (+ 32)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int at = (r & 3) + 8 * (r >> 2);
+        if (at >= left) s0[r] = NEG_INF;
+        if (at + 32 >= left) s1[r] = NEG_INF;
+    }
+}
+
+// ---- values that are infinite or NaN under a mask.  A hidden key's probability is 0, but 0 x inf in the matrix product
+// is NaN in every row of the tile.  Tiles that are masked somewhere are therefore looked through (largest magnitude bits
+// of the tile); a work item that met such a value is computed again, tile by tile, as the product over the finite
+// values, then +-inf (NaN: both) wherever a key with a probability above 0 holds one, found by two products with 0 / 1
+// matrices.
+template <int D>
+__device__ __forceinline__ bool tile_not_finite(const char* sv, int lane) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+    u16x2 mx = {0, 0};
+#pragma unroll
+    for (int i = 0; i < D * BKV * 2 / 1024; ++i) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(sv + i * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
+    }
+    return __any(mx[0] >= 0x7f80 || mx[1] >= 0x7f80);
+}
+
+template <int D, int NW, bool CAP>
+__device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
+                                             char* smem, const Stream<D, NW, true>& kst, const Stream<D, NW, false>& vst, int t,
+                                             int nvis, const Args& a, int wave, int lane) {
+    constexpr int TILE = BKV * D * 2;
+    asm volatile("" : "+v"(lane));      // addresses are derived here again instead of kept in registers all along
+    const int l31 = lane & 31, hi = lane >> 5;
+    kst.stage(t, smem, wave, lane);
+    vst.stage(t, smem + 2 * TILE, wave, lane);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const char* sv = smem + 2 * TILE;
+    f32x16 s0, s1;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s0[j] = s1[j] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        const bf16x8 kf0 = *reinterpret_cast<const bf16x8*>(smem + k_off<D>(l31, 2 * ks + hi));
+        const bf16x8 kf1 = *reinterpret_cast<const bf16x8*>(smem + k_off<D>(32 + l31, 2 * ks + hi));
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf0, qf[ks], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], s1, 0, 0, 0);
+    }
+    if (CAP) {
+        cap_scores(s0, a.cap_in, a.cap_out);
+        cap_scores(s1, a.cap_in, a.cap_out);
+    }
+    mask_scores(s0, s1, t * BKV, nvis, hi);
+    const float sc = CAP ? 1.f : a.scale_log2;
+    float mx = -3.0e38f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = max3(mx, s0[r], s1[r]);
+    const float m_new = __builtin_fmaxf(m_c, half_max(mx) * sc);
+    const float alpha = __builtin_amdgcn_exp2f(m_c - m_new);
+    m_c = m_new;
+    float sum = 0.f;
+    uint32_t pw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const f32x16& c = i < 8 ? s0 : s1;
+        const float pa = __builtin_amdgcn_exp2f(__builtin_fmaf(c[(i & 7) * 2], sc, -m_c));
+        const float pb = __builtin_amdgcn_exp2f(__builtin_fmaf(c[(i & 7) * 2 + 1], sc, -m_c));
+        sum += pa + pb;
+        pw[i] = pack_bf2(pa, pb);
+    }
+    l_run = l_run * alpha + sum;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+        f32x16 pos, neg;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            pos[j] = neg[j] = 0.f;
+            o_acc[db][j] *= alpha;
+        }
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
+            const bf16x8 v = read_v<D>(sv, st, db, lane);
+            bf16x8 fin, vp, vn;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned u = (unsigned short)v[e];
+                const bool bad = (u & 0x7f80u) == 0x7f80u, nan = bad && (u & 0x7fu);
+                fin[e] = bad ? (short)0 : v[e];
+                vp[e] = (nan || u == 0x7f80u) ? (short)0x3f80 : (short)0;
+                vn[e] = (nan || u == 0xff80u) ? (short)0x3f80 : (short)0;
+            }
+            o_acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fin, pf, o_acc[db], 0, 0, 0);
+            pos = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp, pf, pos, 0, 0, 0);
+            neg = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vn, pf, neg, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (pos[j] > 0.f) o_acc[db][j] += __builtin_inff();
+            if (neg[j] > 0.f) o_acc[db][j] -= __builtin_inff();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();          // every wave is done with the tiles
+}
+
+// Step t of a wave: the exponentials, sum and P V of tile t (scores c0 / c1, already computed) while the matrix pipe
+// forms S^T of tile t + 1 in n0 / n1.  K of tile t + 2 and V of tile t + 1 are put in flight from inside.
+// The running maximum m_c is raised only when a tile exceeds it by RESCALE_THR (log2 units): probabilities stay below
+// 2^THR, which costs no relative precision, and most tiles skip the rescale of O.
+template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT>
+__device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
+                                          const f32x16& c0, const f32x16& c1, f32x16& n0, f32x16& n1, float& mx, bool& need,
+                                          const char* sk_next, const char* sv_cur, const Stream<D, NW, true>& kst, char* k_dst,
+                                          bool more_k, const Stream<D, NW, false>& vst, char* v_dst, bool more_v, int t,
+                                          int nvis, bool masked_cur, bool& redo, const Args& a, int wave,
+                                          int lane) {
+    constexpr int DB = D / 32, KS = D / 16;
+    const int l31 = lane & 31, hi = lane >> 5;
+    if (need) {
+        const float m_new = __builtin_fmaxf(m_c, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_c - m_new);
+        m_c = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o_acc[i][j] *= alpha;
+    }
+    if (HAS_NEXT) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) n0[j] = n1[j] = 0.f;
+    }
+    const float sc = CAP ? 1.f : a.scale_log2;
+    float rs0 = 0.f, rs1 = 0.f;
+    uint32_t pw[16];
+#define SOFTMAX_PAIR(i)                                                                                    \
+    do {                                                                                                   \
+        const f32x16& c_ = (i) < 8 ? c0 : c1;                                                              \
+        const int r_ = ((i) & 7) * 2;                                                                      \
+        const float pa_ = __builtin_amdgcn_exp2f(CAP ? c_[r_] - m_c : __builtin_fmaf(c_[r_], sc, -m_c));   \
+        const float pb_ = __builtin_amdgcn_exp2f(CAP ? c_[r_ + 1] - m_c : __builtin_fmaf(c_[r_ + 1], sc, -m_c)); \
+        rs0 += pa_;                                                                                        \
+        rs1 += pb_;                                                                                        \
+        pw[i] = pack_bf2(pa_, pb_);                                                                        \
+        asm volatile("" : "+v"(pw[i]), "+v"(rs0), "+v"(rs1));                                              \
+    } while (0)
+    bf16x8 kf[2][2], vf[2][DB];
+    if (HAS_NEXT) {
+        kf[0][0] = *reinterpret_cast<const bf16x8*>(sk_next + k_off<D>(l31, hi));
+        kf[0][1] = *reinterpret_cast<const bf16x8*>(sk_next + k_off<D>(32 + l31, hi));
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        if (HAS_NEXT) {
+            if (ks < KS - 1) {
+                kf[(ks + 1) & 1][0] = *reinterpret_cast<const bf16x8*>(sk_next + k_off<D>(l31, 2 * ks + 2 + hi));
+                kf[(ks + 1) & 1][1] = *reinterpret_cast<const bf16x8*>(sk_next + k_off<D>(32 + l31, 2 * ks + 2 + hi));
+            }
+            n0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks & 1][0], qf[ks], n0, 0, 0, 0);
+            n1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks & 1][1], qf[ks], n1, 0, 0, 0);
+        }
+        if constexpr (D == 128) {
+            SOFTMAX_PAIR(ks);
+        } else {
+            SOFTMAX_PAIR(2 * ks);
+            SOFTMAX_PAIR(2 * ks + 1);
+        }
+        if (ks == 0 && more_k) kst.stage(t + 2, k_dst, wave, lane);
+        if (ks == 1 && more_v) vst.stage(t + 1, v_dst, wave, lane);
+        if (ks == KS - 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) vf[0][db] = read_v<D>(sv_cur, 0, db, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (HAS_NEXT && CAP) {
+        cap_scores(n0, a.cap_in, a.cap_out);
+        cap_scores(n1, a.cap_in, a.cap_out);
+    }
+    if (HAS_NEXT && MASK_NEXT) mask_scores(n0, n1, (t + 1) * BKV, nvis, hi);
+    float nmx = -3.0e38f;
+    const float sc_next = CAP ? 1.f : a.scale_log2;
+    if ((MASK_NEXT || !HAS_NEXT) && masked_cur) redo |= tile_not_finite<D>(sv_cur, lane);
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+        if (st < 3) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) vf[(st + 1) & 1][db] = read_v<D>(sv_cur, st + 1, db, lane);
+        }
+        const bf16x8 pfrag =
+            __builtin_bit_cast(bf16x8, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+            o_acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[st & 1][db], pfrag, o_acc[db], 0, 0, 0);
+        if (st == 0) { SOFTMAX_PAIR(8); SOFTMAX_PAIR(9); SOFTMAX_PAIR(10); }
+        if (st == 1) { SOFTMAX_PAIR(11); SOFTMAX_PAIR(12); SOFTMAX_PAIR(13); }
+        if (st == 2) { SOFTMAX_PAIR(14); SOFTMAX_PAIR(15); }
+        if (st >= 2 && HAS_NEXT) {
+            const f32x16& n = st == 2 ? n0 : n1;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) nmx = max3(nmx, n[r], n[r + 1]);
+            asm volatile("" : "+v"(nmx));
+            if (st == 3) {
+                mx = half_max(nmx) * sc_next;
+                need = __any(mx > m_c + RESCALE_THR);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    l_run += rs0 + rs1;
+#undef SOFTMAX_PAIR
+}
+
 // one work item: 32 NW rows of document `doc` under key head kvh, keys of split `split`
 template <int D, int NW, bool CAP>
 __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int split, int doc, int rb) {
     constexpr int ROWB = D * 2;                          // bytes per K / V row
-    constexpr int TILE = BKV * ROWB;                     // bytes per tile
+    constexpr int TILE = BKV * ROWB;                     // bytes per tile; LDS: K[2] | V[2]
     constexpr int CPR = ROWB / 16;                       // chunks per row
     constexpr int RPI = 64 / CPR;                        // rows per DMA instruction of a wave
     constexpr int DB = D / 32, KS = D / 16;
@@ -145,13 +418,16 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
     const long row = min(r_first + l31, rows - 1);       // rows past the last repeat it and are not stored
     const int tok = (int)(row / a.group), head = kvh * a.group + (int)(row % a.group);
     const int nvis = visible(a, tok, lq, lk, prefix);
-    // visible counts grow with the row: the tile range follows from the workgroup's last row, the tiles that need no
-    // mask from the wave's first
+    // visible counts grow with the row: the tile range follows from the workgroup's last row; a wave's own last row says
+    // where its work ends, its first row which tiles need no mask
     const long last_row = min((long)(rb + 1) * (32 * NW), rows) - 1;
-    const int kend = visible(a, (int)(last_row / a.group), lq, lk, prefix);
-    const int full = visible(a, (int)(min(r_first, rows - 1) / a.group), lq, lk, prefix);
+    const int kend = __builtin_amdgcn_readfirstlane(visible(a, (int)(last_row / a.group), lq, lk, prefix));
+    const int wend = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first + 31, rows - 1) / a.group), lq, lk, prefix));
+    const int full = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first, rows - 1) / a.group), lq, lk, prefix));
     const int nt = (kend + BKV - 1) / BKV;
     const int t0 = (int)((long)nt * split / a.n_splits), t1 = (int)((long)nt * (split + 1) / a.n_splits);
+    const int tw = min(max((wend + BKV - 1) / BKV, t0), t1);     // this wave's tiles: [t0, tw)
+    const int tf = min(max(full / BKV, t0), tw);                 // ... of which [t0, tf) are seen whole by all its rows
 
     bf16x8 qf[KS];
     {
@@ -159,102 +435,110 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
     }
-    const char* kb = reinterpret_cast<const char*>(a.k + (long)k0 * a.k_ld + (long)kvh * D);
-    const char* vb = reinterpret_cast<const char*>(a.v + (long)k0 * a.v_ld + (long)kvh * D);
-    auto stage = [&](int t, int buf) {
-        char* dst = smem + buf * 2 * TILE;
-#pragma unroll
-        for (int i = 0; i < TILE / 1024 / NW; ++i) {
-            const int r = (i * NW + wave) * RPI + lane / CPR, c = lane % CPR;
-            const long key = min(t * BKV + r, lk - 1);
-            const int ck = D == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
-            const int cv = D == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
-            __builtin_amdgcn_global_load_lds(kb + key * a.k_ld * 2 + ck * 16, (lds_ptr)(dst + (i * NW + wave) * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(vb + key * a.v_ld * 2 + cv * 16, (lds_ptr)(dst + TILE + (i * NW + wave) * 1024), 16, 0, 0);
-        }
-    };
+    Stream<D, NW, true> kst;
+    Stream<D, NW, false> vst;
+    kst.init(a.k + (long)k0 * a.k_ld + (long)kvh * D, a.k_ld, lk, wave, lane);
+    vst.init(a.v + (long)k0 * a.v_ld + (long)kvh * D, a.v_ld, lk, wave, lane);
     f32x16 o_acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o_acc[i][j] = 0.f;
-    float m_run = NEG_INF, l_run = 0.f;
-    if (t0 < t1) stage(t0, 0);
-    for (int t = t0; t < t1; ++t) {
+    // the running maximum starts at a finite number below every finite score: a row that has seen no key yet has
+    // p = exp2(-inf - m) = 0 with no special case
+    float m_c = -3.0e38f, l_run = 0.f;
+    bool redo = false;
+    if (t0 < t1) {
+        kst.stage(t0, smem, wave, lane);
+        vst.stage(t0, smem + 2 * TILE, wave, lane);
+        if (t0 + 1 < t1) kst.stage(t0 + 1, smem + TILE, wave, lane);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                      // tile t has landed everywhere, every wave is done with tile t - 1
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) stage(t + 1, buf ^ 1);
-        const char* sk = smem + buf * 2 * TILE;
-        const char* sv = sk + TILE;
-        f32x16 s0, s1;
+        __syncthreads();
+        f32x16 a0, a1, b0, b1;
+        float mx = -3.0e38f;
+        bool need = false;
+        if (t0 < tw) {       // scores of the first tile
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s0[j] = s1[j] = 0.f;
+            for (int j = 0; j < 16; ++j) a0[j] = a1[j] = 0.f;
+            const char* sk = smem;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 kf0 = *reinterpret_cast<const bf16x8*>(sk + k_off<D>(l31, 2 * ks + hi));
-            const bf16x8 kf1 = *reinterpret_cast<const bf16x8*>(sk + k_off<D>(32 + l31, 2 * ks + hi));
-            s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf0, qf[ks], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], s1, 0, 0, 0);
-        }
-        // scores in units of log2: s * scale * log2(e), or cap log2(e) tanh(s scale / cap) with
-        // tanh(x) = 1 - 2 / (1 + e^2x) (both ends saturate without overflow)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if constexpr (CAP) {
-                s0[j] = a.cap_out - 2.f * a.cap_out * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s0[j] * a.cap_in));
-                s1[j] = a.cap_out - 2.f * a.cap_out * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s1[j] * a.cap_in));
-            } else {
-                s0[j] *= a.scale_log2;
-                s1[j] *= a.scale_log2;
+            for (int ks = 0; ks < KS; ++ks) {
+                const bf16x8 kf0 = *reinterpret_cast<const bf16x8*>(sk + k_off<D>(l31, 2 * ks + hi));
+                const bf16x8 kf1 = *reinterpret_cast<const bf16x8*>(sk + k_off<D>(32 + l31, 2 * ks + hi));
+                a0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf0, qf[ks], a0, 0, 0, 0);
+                a1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], a1, 0, 0, 0);
             }
-        }
-        if ((t + 1) * BKV > full) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int key = t * BKV + (r & 3) + 8 * (r >> 2) + 4 * hi;
-                if (key >= nvis) s0[r] = NEG_INF;
-                if (key + 32 >= nvis) s1[r] = NEG_INF;
+            if (CAP) {
+                cap_scores(a0, a.cap_in, a.cap_out);
+                cap_scores(a1, a.cap_in, a.cap_out);
             }
+            if (t0 >= tf) mask_scores(a0, a1, t0 * BKV, nvis, hi);
+            float nmx = -3.0e38f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) nmx = max3(nmx, a0[r], a1[r]);
+            mx = half_max(nmx) * (CAP ? 1.f : a.scale_log2);
+            need = __any(mx > m_c + RESCALE_THR);
         }
-        float mx = s0[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = __builtin_fmaxf(mx, s0[r]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s1[r]);
-        const float m_new = __builtin_fmaxf(m_run, half_max(mx));
-        const float m_ref = m_new == NEG_INF ? 0.f : m_new;       // no key seen yet: every p is exp2(-inf) = 0
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
-        m_run = m_new;
-        float sum = 0.f;
-        uint32_t pw[16];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float a0 = __builtin_amdgcn_exp2f(s0[2 * i] - m_ref), a1 = __builtin_amdgcn_exp2f(s0[2 * i + 1] - m_ref);
-            const float b0 = __builtin_amdgcn_exp2f(s1[2 * i] - m_ref), b1 = __builtin_amdgcn_exp2f(s1[2 * i + 1] - m_ref);
-            sum += (a0 + a1) + (b0 + b1);
-            pw[i] = pack_bf2(a0, a1);
-            pw[8 + i] = pack_bf2(b0, b1);
+        __syncthreads();      // every wave is done with K(t0) before K(t0 + 2) overwrites it
+        // step u handles tile t0 + u; buffers go by the parity of u.  LDS during it: K of the next tile, V of this one
+#define PIPE_STEP(HAS_NEXT, MASK_NEXT, C0, C1, N0, N1, U)                                                           \
+    do {                                                                                                            \
+        const int u_ = (U), t_ = t0 + u_;                                                                           \
+        pipe_step<D, NW, CAP, HAS_NEXT, MASK_NEXT>(o_acc, qf, m_c, l_run, C0, C1, N0, N1, mx, need,                 \
+                                                   smem + ((u_ + 1) & 1) * TILE, smem + (2 + (u_ & 1)) * TILE, kst, \
+                                                   smem + (u_ & 1) * TILE, t_ + 2 < t1, vst,                        \
+                                                   smem + (2 + ((u_ + 1) & 1)) * TILE, t_ + 1 < t1, t_, nvis,       \
+                                                   t_ >= tf, redo, a, wave, lane);                                  \
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                            \
+        __syncthreads();                                                                                            \
+    } while (0)
+        int u = 0;
+        for (; t0 + u + 2 < tf; u += 2) {     // next tile whole; two steps per turn: the score registers swap roles
+            PIPE_STEP(true, false, a0, a1, b0, b1, u);
+            PIPE_STEP(true, false, b0, b1, a0, a1, u + 1);
         }
-        l_run = l_run * alpha + sum;
+        if (t0 + u + 1 < tf) {
+            PIPE_STEP(true, false, a0, a1, b0, b1, u);
+            a0 = b0;
+            a1 = b1;
+            ++u;
+        }
+        for (; t0 + u + 1 < tw; ++u) {
+            PIPE_STEP(true, true, a0, a1, b0, b1, u);
+            a0 = b0;
+            a1 = b1;
+        }
+        if (t0 + u < tw) {
+            PIPE_STEP(false, false, a0, a1, b0, b1, u);
+            ++u;
+        }
+#undef PIPE_STEP
+        for (; t0 + u < t1; ++u) {            // rows of other waves still see keys: keep their tiles coming
+            if (t0 + u + 2 < t1) kst.stage(t0 + u + 2, smem + (u & 1) * TILE, wave, lane);
+            if (t0 + u + 1 < t1) vst.stage(t0 + u + 1, smem + (2 + ((u + 1) & 1)) * TILE, wave, lane);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+    }
+    // rows of the workgroup see different key counts: only then can a hidden value have been multiplied
+    const int wfull = __builtin_amdgcn_readfirstlane(visible(a, (int)((long)rb * (32 * NW) / a.group), lq, lk, prefix));
+    if (t1 > wfull / BKV && t0 < t1) {
+        int* flags = reinterpret_cast<int*>(smem);        // the tiles are free (last step's barrier)
+        if (lane == 0) flags[wave] = redo;
+        __syncthreads();
+        int any = 0;
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
+        for (int w = 0; w < NW; ++w) any |= flags[w];
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(any)) {
+            m_c = -3.0e38f;
+            l_run = 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o_acc[i][j] *= alpha;
-        const int g = lane >> 4, i16 = lane & 15, qd = i16 >> 2, pp = i16 & 3;
+            for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pw[4 * st], pw[4 * st + 1], pw[4 * st + 2], pw[4 * st + 3]));
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                const int kr = 16 * st + 4 * (g >> 1) + qd;
-                const int ch = db * 4 + 2 * (g & 1) + (pp >> 1);
-                const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4_ptr)(sv + v_off<D>(kr, ch) + 8 * (pp & 1)));
-                const bf16x4_t h4 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4_ptr)(sv + v_off<D>(kr + 8, ch) + 8 * (pp & 1)));
-                const uint2 lo2 = __builtin_bit_cast(uint2, lo), hi2 = __builtin_bit_cast(uint2, h4);
-                const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
-                o_acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o_acc[db], 0, 0, 0);
-            }
+                for (int j = 0; j < 16; ++j) o_acc[i][j] = 0.f;
+            for (int t = t0; t < t1; ++t)
+                careful_step<D, NW, CAP>(o_acc, qf, m_c, l_run, smem, kst, vst, t, nvis, a, wave, lane);
         }
     }
     l_run = half_sum(l_run);
@@ -270,11 +554,11 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
             for (int g4 = 0; g4 < 4; ++g4)
                 *reinterpret_cast<float4*>(w + db * 32 + 8 * g4) =
                     make_float4(o_acc[db][4 * g4], o_acc[db][4 * g4 + 1], o_acc[db][4 * g4 + 2], o_acc[db][4 * g4 + 3]);
-        if (hi == 0) *reinterpret_cast<float2*>(ws_stat<D>(a, split, wrow)) = make_float2(m_run, l_run);
+        if (hi == 0) *reinterpret_cast<float2*>(ws_stat<D>(a, split, wrow)) = make_float2(m_c, l_run);
         return;
     }
     const float inv = l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run);     // no key: 0; NaN stays NaN
-    __syncthreads();                          // the tiles are free: 64 D bytes per wave for the output rows
+    // the tiles are free (last step's barrier): 64 D bytes per wave for the output rows
     char* ep = smem + wave * (64 * D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -295,20 +579,30 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
     }
 }
 
-// The grid holds `row_blocks` work items per key head and split, enough for the lengths the host was told; should the
-// documents be longer than that, a workgroup goes on with the items a grid further.
+// The grid holds `row_blocks` work items per key head and split: never fewer than the documents need, whatever their
+// lengths (sum of ceil(rows / per) <= total / per + documents); the rest find nothing to do.
 template <int D, int NW, bool CAP>
-__global__ void __launch_bounds__(64 * NW) attn_packed_kernel(Args a) {
+__global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_kernel(Args a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];   // (K | V)[2]
+    // Workgroup ids go round-robin over the 8 XCDs, each with its own L2: a key head is served by one XCD (heads a multiple
+    // of 8), or every XCD takes one contiguous range of the (head, row block) space.
     const int split = blockIdx.x % a.n_splits, id = blockIdx.x / a.n_splits;
-    const int kvh = id / a.row_blocks;
-    for (int blk = id % a.row_blocks;; blk += a.row_blocks) {
-        int doc, rb, left;
-        if (!find_block<32 * NW>(a, blk, threadIdx.x & 63, doc, rb, left)) return;
-        attend<D, NW, CAP>(a, smem, kvh, split, __builtin_amdgcn_readfirstlane(doc), __builtin_amdgcn_readfirstlane(rb));
-        if (__builtin_amdgcn_readfirstlane(left) < a.row_blocks) return;
-        __syncthreads();                      // the output staging of this item before the tiles of the next
+    int kvh, blk;
+    if (a.n_splits == 1 && (a.kv_heads & 7) == 0) {
+        kvh = (id & 7) + 8 * ((id >> 3) / a.row_blocks);
+        blk = (id >> 3) % a.row_blocks;
+    } else if (a.n_splits == 1) {
+        const int total = a.kv_heads * a.row_blocks, xcd = id & 7, q = total >> 3, r = total & 7;
+        const int lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+        kvh = lin / a.row_blocks;
+        blk = lin % a.row_blocks;
+    } else {
+        kvh = id / a.row_blocks;
+        blk = id % a.row_blocks;
     }
+    int doc, rb;
+    if (!find_block<32 * NW>(a, blk, threadIdx.x & 63, doc, rb)) return;
+    attend<D, NW, CAP>(a, smem, kvh, split, __builtin_amdgcn_readfirstlane(doc), __builtin_amdgcn_readfirstlane(rb));
 }
 
 // out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the splits, in their order; one wave per (token, head), rows
@@ -321,13 +615,12 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
     if (row >= (long)a.total_q * heads) return;
     const int tok = (int)(row / heads), head = (int)(row % heads);
     if (tok < a.cu_q[0] || tok >= a.cu_q[a.docs]) return;
-    float m = NEG_INF;
+    float m = -3.0e38f;
     for (int s = 0; s < a.n_splits; ++s) m = __builtin_fmaxf(m, ws_stat<D>(a, s, row)[0]);
-    const float m_ref = m == NEG_INF ? 0.f : m;
     float l = 0.f, o0 = 0.f, o1 = 0.f;
     for (int s = 0; s < a.n_splits; ++s) {
         const float2 st = *reinterpret_cast<const float2*>(ws_stat<D>(a, s, row));
-        const float w = __builtin_amdgcn_exp2f(st.x - m_ref);
+        const float w = __builtin_amdgcn_exp2f(st.x - m);
         const float* p = ws_row<D>(a, s, row);
         l = fmaf(st.y, w, l);
         if constexpr (D == 128) {
@@ -354,12 +647,10 @@ Plan plan_of(long total_q, int docs, int kv_heads, int group, long max_q, long m
     Plan p;
     max_q = max_q < 1 ? 1 : (max_q > total_q ? total_q : max_q);
     const long rows = max_q * group;
-    p.waves = rows <= 32 ? 1 : 4;
+    // 256-row workgroups when they fill the chip, 128 rows otherwise
+    p.waves = rows <= 32 ? 1 : (total_q * group / 256 * kv_heads >= ovd_device_cus() ? 8 : 4);
     const long per = 32L * p.waves;
-    // sum over documents of ceil(Lq group / per) <= total / per + docs, and <= docs * ceil(max / per)
-    long nb = total_q * group / per + docs;
-    const long nb2 = docs * ((rows + per - 1) / per);
-    p.row_blocks = (int)(nb < nb2 ? nb : nb2);
+    p.row_blocks = (int)(total_q * group / per + docs);        // >= the sum of ceil(Lq group / per) over the documents
     p.splits = 1;
     const long wgs = (long)p.row_blocks * kv_heads;
     if (p.waves == 1 && wgs < 2L * ovd_device_cus()) {
@@ -396,6 +687,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
                 "attn_packed: token rows must keep 16-byte alignment");
     OVD_REQUIRE(q_ld >= (long)q_heads * D && o_ld >= (long)q_heads * D && k_ld >= (long)kv_heads * D && v_ld >= (long)kv_heads * D,
                 "attn_packed: token stride shorter than the heads");
+    OVD_REQUIRE(k_ld < (1L << 24) && v_ld < (1L << 24), "attn_packed: token stride too long");
     OVD_REQUIRE(softmax_scale > 0.f && softcap >= 0.f && softmax_scale < 1e30f && softcap < 1e30f,
                 "attn_packed: softmax_scale must be positive, softcap positive or 0 (none)");
     OVD_REQUIRE(prefix == nullptr || causal, "attn_packed: a prefix goes with the causal mask");
@@ -432,6 +724,8 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     {                                                                   \
         if (p.waves == 1) {                                             \
             if (softcap > 0.f) PACKED(DD, 1, true) else PACKED(DD, 1, false) \
+        } else if (p.waves == 8) {                                      \
+            if (softcap > 0.f) PACKED(DD, 8, true) else PACKED(DD, 8, false) \
         } else {                                                        \
             if (softcap > 0.f) PACKED(DD, 4, true) else PACKED(DD, 4, false) \
         }                                                               \

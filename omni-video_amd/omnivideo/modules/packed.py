@@ -86,7 +86,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=Fa
     first max(i + Lk - Lq + 1, prefix[d]) of them (prefix int32 [documents] or None).  softcap > 0 caps the scores:
     softcap * tanh(s / softcap).  softmax_scale defaults to D ** -0.5.
     A query that sees no key gets zeros.  Rows outside every document are not written (uninitialised when `out` is not
-    given).  Values of keys that a causal mask hides inside a document must be finite (they are weighted by zero).
+    given).  A key that is hidden from a query does not enter its result, whatever it and its value hold.
     max_q, max_k: the longest document as the caller knows it (default: the totals); they size the launch, any value
     gives right results.  workspace: a byte buffer of H.attn_packed_workspace_bytes(...) (default: allocated here)."""
     _no_grad(q, k, v)

@@ -258,6 +258,33 @@ def test_attention_outside_a_document_nothing_is_read_or_written(P):
             assert torch.isnan(out[3 + Lq[0]:-9]).all()
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lq,Lk,N,Nk", [([300], [300], 2, 2), ([1, 3], [700, 900], 8, 1), ([700, 130], [720, 140], 4, 2)])
+def test_attention_infinities_and_nan_under_the_causal_mask(P, Lq, Lk, N, Nk, D):
+    """what a hidden key and its value hold does not enter a row; a row that sees it gets the infinity or NaN"""
+    q, k, v = inputs(Lq, Lk, N, Nk, D, 77)
+    want, bound = ref_attention(q, k, v, Lq, Lk, True, None, 0.0, D ** -0.5)
+    bad = Lk[0] - 2                                    # seen by the last two queries of the first document
+    q0 = Lq[0]
+    hidden = max(q0 - 2, 0)
+    for value in (math.nan, math.inf, -math.inf):
+        vv = v.clone()
+        vv[bad, 0, 5], vv[bad, 0, D - 1] = value, value
+        o = P.packed_attention(q, k, vv, cu(Lq), cu(Lk), max(Lq), max(Lk), causal=True)
+        heads = N // Nk
+        assert torch.isfinite(o[hidden:q0, :, 6:D - 1]).all()
+        seen = o[hidden:q0, :heads, [5, D - 1]].float()
+        assert torch.isnan(seen).all() if math.isnan(value) else bool((seen == value).all())
+        o[hidden:q0, :heads, [5, D - 1]] = want[hidden:q0, :heads, [5, D - 1]].to(BF16)
+        check(o, want, bound)
+    kk = k.clone()
+    kk[bad] = math.nan
+    o = P.packed_attention(q, kk, v, cu(Lq), cu(Lk), max(Lq), max(Lk), causal=True)
+    assert torch.isnan(o[hidden:q0]).all()
+    o[hidden:q0] = want[hidden:q0].to(BF16)
+    check(o, want, bound)
+
+
 def test_attention_strided_views_of_a_fused_projection(P):
     T, N, D = 333, 4, 128
     buf = randn((T, 3 * N * D + 8), 21)
