@@ -358,8 +358,8 @@ int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos
  * ovd_attn_packed_workspace_bytes(...) (HOST) bytes, 16-byte aligned; NULL or smaller: not split.  It holds no state
  * between calls; calls that may overlap need their own.
  * The reference packs a padded batch this way for flash_attn_varlen_func (omnivideo/modules/attention.py:96-130). */
-int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int docs, int q_heads, int kv_heads, int head_dim, int64_t max_q,
-                                        int64_t max_k);
+int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int64_t total_k, int docs, int q_heads, int kv_heads, int head_dim,
+                                        int64_t max_q, int64_t max_k);
 int ovd_attn_packed_fwd_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int64_t total_q,
                              int64_t total_k, const int32_t* cu_q, const int32_t* cu_k, int docs, int64_t max_q,
                              int64_t max_k, int q_heads, int kv_heads, int head_dim, int64_t q_ld, int64_t k_ld,

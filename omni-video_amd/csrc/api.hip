@@ -51,7 +51,7 @@ int ovd_impl_linear_mxfp4(const void*, int, long, const uint8_t*, const uint8_t*
                           void*, long, int, int, int, int, hipStream_t);
 int ovd_impl_rope_positions(const void*, int, long, const void*, int, int, const double*, const int*, void*, long, long,
                             int, int, int, int, hipStream_t);
-long ovd_impl_attn_packed_workspace(long, int, int, int, int, long, long);
+long ovd_impl_attn_packed_workspace(long, long, int, int, int, int, long, long);
 int ovd_impl_attn_packed(const bf16_t*, const bf16_t*, const bf16_t*, bf16_t*, long, long, const int*, const int*, int, long,
                          long, int, int, int, long, long, long, long, int, const int*, float, float, void*, long,
                          hipStream_t);
@@ -376,9 +376,9 @@ int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos
                                    head_dim, interleaved, inverse, ST(stream));
 }
 
-int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int docs, int q_heads, int kv_heads, int head_dim, int64_t max_q,
-                                        int64_t max_k) {
-    return ovd_impl_attn_packed_workspace(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k);
+int64_t ovd_attn_packed_workspace_bytes(int64_t total_q, int64_t total_k, int docs, int q_heads, int kv_heads, int head_dim,
+                                        int64_t max_q, int64_t max_k) {
+    return ovd_impl_attn_packed_workspace(total_q, total_k, docs, q_heads, kv_heads, head_dim, max_q, max_k);
 }
 
 int ovd_attn_packed_fwd_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int64_t total_q,

@@ -14,7 +14,7 @@
 // Lq * group rows; a workgroup of NW waves takes 32 NW of them, 32 per wave, so a single token's group of heads fills a
 // tile together and K / V are read once per group.  Which document a workgroup serves follows from cu_q on the device
 // (a wave-wide scan), so lengths can change under a captured graph; the grid is the largest that the shapes allow.
-// Few rows against long documents: n_splits workgroups share the keys of a tile and a second kernel joins them.
+// Few rows: the keys of long documents are split into parts and a second kernel joins them.
 //
 // S^T = K Q^T with the key on the MFMA row axis (v_mfma_f32_32x32x16_bf16): a lane holds 32 scores of ONE query, so row
 // maxima and sums are in-lane plus one exchange, and P is already the B operand of O^T += V^T P^T.  V^T fragments come
@@ -61,8 +61,9 @@ struct Args {
     int total_q, total_k, docs, kv_heads, group, causal;
     float scale_log2;                         // softmax scale * log2(e)
     float cap_in, cap_out;                    // 2 scale log2(e) / cap, cap log2(e)  (capped form)
-    int row_blocks, n_splits;
-    float* ws;                                // partial results of the splits
+    int row_blocks;
+    int chunk, max_splits;                    // split form: key tiles a work item should have, most parts of a document
+    float* ws;                                // partial results of the parts
 };
 
 // rows [*q0, *q0 + *lq) and keys [*k0, *k0 + *lk) of document d; whatever cu_q / cu_k hold, inside the tensors
@@ -73,16 +74,26 @@ __device__ __forceinline__ void doc_range(const Args& a, int d, int& q0, int& lq
     lk = min(max(a.cu_k[d + 1], k0), a.total_k) - k0;
 }
 
-// document and row block (of ROWS rows) of work item `blk`; false past the last one
-template <int ROWS>
-__device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int& doc, int& rb) {
+// parts into which the keys of a document of lk keys are split
+__device__ __forceinline__ int parts_of(const Args& a, int lk) {
+    const int nt = (lk + BKV - 1) / BKV;
+    return min(max((nt + a.chunk - 1) / a.chunk, 1), a.max_splits);
+}
+
+// document, row block (of ROWS rows) and part of its keys of work item `blk`; false past the last one
+template <int ROWS, bool SPLIT>
+__device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int& doc, int& rb, int& part, int& parts) {
     for (int d0 = 0; d0 < a.docs; d0 += 64) {
         const int d = d0 + lane;
-        int n = 0;
+        int n = 0, np = 1;
         if (d < a.docs) {
-            const int q0 = min(max(a.cu_q[d], 0), a.total_q);
-            const int lq = min(max(a.cu_q[d + 1], q0), a.total_q) - q0;
+            int q0, lq, k0, lk;
+            doc_range(a, d, q0, lq, k0, lk);
             n = (int)(((long)lq * a.group + ROWS - 1) / ROWS);
+            if (SPLIT) {
+                np = parts_of(a, lk);
+                n *= np;
+            }
         }
         int incl = n;
 #pragma unroll
@@ -95,7 +106,14 @@ __device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int
             const int l = __builtin_ctzll(hit);
             doc = d0 + l;
             rb = blk - __shfl(incl - n, l, 64);
-            if (a.causal) rb = __shfl(n, l, 64) - 1 - rb;          // the longest rows first
+            if (a.causal && !SPLIT) rb = __shfl(n, l, 64) - 1 - rb;          // the longest rows first
+            part = 0;
+            parts = 1;
+            if (SPLIT) {
+                parts = __shfl(np, l, 64);
+                part = rb % parts;
+                rb /= parts;
+            }
             return true;
         }
         blk -= __shfl(incl, 63, 64);
@@ -109,16 +127,16 @@ __device__ __forceinline__ int visible(const Args& a, int i, int lq, int lk, int
     return min(max(n, 0), lk);
 }
 
-// workspace: accumulators [n_splits][rows = total_q * Nq][D], then (maximum, sum) [n_splits][rows][2]
+// workspace: accumulators [max_splits][rows = total_q * Nq][D], then (maximum, sum) [max_splits][rows][2]
 template <int D>
-__device__ __forceinline__ float* ws_row(const Args& a, int split, long row) {
+__device__ __forceinline__ float* ws_row(const Args& a, int part, long row) {
     const long rows = (long)a.total_q * a.kv_heads * a.group;
-    return a.ws + (split * rows + row) * D;
+    return a.ws + (part * rows + row) * D;
 }
 template <int D>
-__device__ __forceinline__ float* ws_stat(const Args& a, int split, long row) {
+__device__ __forceinline__ float* ws_stat(const Args& a, int part, long row) {
     const long rows = (long)a.total_q * a.kv_heads * a.group;
-    return a.ws + a.n_splits * rows * D + (split * rows + row) * 2;
+    return a.ws + a.max_splits * rows * D + (part * rows + row) * 2;
 }
 
 // DMA of one operand: 64-row tiles HBM -> LDS.  A wave's instruction covers RPI rows; rows past the document's last key
@@ -399,9 +417,9 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
 #undef SOFTMAX_PAIR
 }
 
-// one work item: 32 NW rows of document `doc` under key head kvh, keys of split `split`
-template <int D, int NW, bool CAP>
-__device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int split, int doc, int rb) {
+// one work item: 32 NW rows of document `doc` under key head kvh, part `part` of `parts` of their keys
+template <int D, int NW, bool CAP, bool SPLIT>
+__device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int doc, int rb, int part, int parts) {
     constexpr int ROWB = D * 2;                          // bytes per K / V row
     constexpr int TILE = BKV * ROWB;                     // bytes per tile; LDS: K[2] | V[2]
     constexpr int CPR = ROWB / 16;                       // chunks per row
@@ -425,7 +443,7 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
     const int wend = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first + 31, rows - 1) / a.group), lq, lk, prefix));
     const int full = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first, rows - 1) / a.group), lq, lk, prefix));
     const int nt = (kend + BKV - 1) / BKV;
-    const int t0 = (int)((long)nt * split / a.n_splits), t1 = (int)((long)nt * (split + 1) / a.n_splits);
+    const int t0 = (int)((long)nt * part / parts), t1 = (int)((long)nt * (part + 1) / parts);
     const int tw = min(max((wend + BKV - 1) / BKV, t0), t1);     // this wave's tiles: [t0, tw)
     const int tf = min(max(full / BKV, t0), tw);                 // ... of which [t0, tf) are seen whole by all its rows
 
@@ -544,17 +562,17 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
     l_run = half_sum(l_run);
     const bool live = r_first + l31 < rows;
     // register j of o_acc[db] is dimension 32 db + 8 (j >> 2) + 4 hi + (j & 3) of query row l31
-    if (a.n_splits > 1) {
+    if (SPLIT && parts > 1) {
         if (!live) return;
         const long wrow = (long)(q0 + tok) * a.kv_heads * a.group + head;
-        float* w = ws_row<D>(a, split, wrow) + 4 * hi;
+        float* w = ws_row<D>(a, part, wrow) + 4 * hi;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4)
                 *reinterpret_cast<float4*>(w + db * 32 + 8 * g4) =
                     make_float4(o_acc[db][4 * g4], o_acc[db][4 * g4 + 1], o_acc[db][4 * g4 + 2], o_acc[db][4 * g4 + 3]);
-        if (hi == 0) *reinterpret_cast<float2*>(ws_stat<D>(a, split, wrow)) = make_float2(m_c, l_run);
+        if (hi == 0) *reinterpret_cast<float2*>(ws_stat<D>(a, part, wrow)) = make_float2(m_c, l_run);
         return;
     }
     const float inv = l_run > 0.f ? 1.f / l_run : (l_run == l_run ? 0.f : l_run);     // no key: 0; NaN stays NaN
@@ -579,34 +597,55 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int s
     }
 }
 
-// The grid holds `row_blocks` work items per key head and split: never fewer than the documents need, whatever their
-// lengths (sum of ceil(rows / per) <= total / per + documents); the rest find nothing to do.
+// The grid holds `row_blocks` work items per key head: never fewer than the documents need, whatever their lengths
+// (sum of ceil(rows / per) <= total / per + documents); the rest find nothing to do.  Workgroup ids go round-robin over
+// the 8 XCDs, each with its own L2: a key head is served by one XCD (heads a multiple of 8), or every XCD takes one
+// contiguous range of the (head, row block) space.
 template <int D, int NW, bool CAP>
-__global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_kernel(Args a) {
+__global__ void __launch_bounds__(64 * NW, 2) attn_packed_kernel(Args a) {
+#ifdef __HIP_DEVICE_COMPILE__     // the host pass has no use for the body (and refuses register constraints in shared parts of it)
     extern __shared__ __attribute__((aligned(16))) char smem[];   // (K | V)[2]
-    // Workgroup ids go round-robin over the 8 XCDs, each with its own L2: a key head is served by one XCD (heads a multiple
-    // of 8), or every XCD takes one contiguous range of the (head, row block) space.
-    const int split = blockIdx.x % a.n_splits, id = blockIdx.x / a.n_splits;
+    const int id = blockIdx.x;
     int kvh, blk;
-    if (a.n_splits == 1 && (a.kv_heads & 7) == 0) {
+    if ((a.kv_heads & 7) == 0) {
         kvh = (id & 7) + 8 * ((id >> 3) / a.row_blocks);
         blk = (id >> 3) % a.row_blocks;
-    } else if (a.n_splits == 1) {
+    } else {
         const int total = a.kv_heads * a.row_blocks, xcd = id & 7, q = total >> 3, r = total & 7;
         const int lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
         kvh = lin / a.row_blocks;
         blk = lin % a.row_blocks;
-    } else {
-        kvh = id / a.row_blocks;
-        blk = id % a.row_blocks;
     }
-    int doc, rb;
-    if (!find_block<32 * NW>(a, blk, threadIdx.x & 63, doc, rb)) return;
-    attend<D, NW, CAP>(a, smem, kvh, split, __builtin_amdgcn_readfirstlane(doc), __builtin_amdgcn_readfirstlane(rb));
+    int doc, rb, part, parts;
+    if (!find_block<32 * NW, false>(a, blk, threadIdx.x & 63, doc, rb, part, parts)) return;
+    doc = __builtin_amdgcn_readfirstlane(doc);
+    rb = __builtin_amdgcn_readfirstlane(rb);
+    attend<D, NW, CAP, false>(a, smem, kvh, doc, rb, 0, 1);
+#endif
 }
 
-// out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the splits, in their order; one wave per (token, head), rows
-// inside [cu_q[0], cu_q[docs]) only
+// Few query rows: the keys of a document are split into parts of about `chunk` tiles, all of one size per document, so
+// that documents of very different lengths fill the chip evenly.  Workgroups go on with further items a grid away: the
+// host sizes the grid by the lengths that it was told.  A document in one part is finished here, the others by the join.
+template <int D, int NW, bool CAP>
+__global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_split_kernel(Args a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int kvh = blockIdx.x % a.kv_heads;
+    for (int blk = blockIdx.x / a.kv_heads;; blk += a.row_blocks) {
+        int doc, rb, part, parts;
+        if (!find_block<32 * NW, true>(a, blk, threadIdx.x & 63, doc, rb, part, parts)) return;
+        doc = __builtin_amdgcn_readfirstlane(doc);
+        rb = __builtin_amdgcn_readfirstlane(rb);
+        part = __builtin_amdgcn_readfirstlane(part);
+        parts = __builtin_amdgcn_readfirstlane(parts);
+        attend<D, NW, CAP, true>(a, smem, kvh, doc, rb, part, parts);
+        __syncthreads();                      // the output staging of this item before the tiles of the next
+    }
+#endif
+}
+
+// out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts, in their order; one wave per (token, head)
 template <int D>
 __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
     const int lane = threadIdx.x & 63;
@@ -614,11 +653,25 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
     const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= (long)a.total_q * heads) return;
     const int tok = (int)(row / heads), head = (int)(row % heads);
-    if (tok < a.cu_q[0] || tok >= a.cu_q[a.docs]) return;
+    int parts = 1;
+    for (int d0 = 0; d0 < a.docs; d0 += 64) {            // the token's document
+        const int d = min(d0 + lane, a.docs - 1);
+        int q0, lq, k0, lk;
+        doc_range(a, d, q0, lq, k0, lk);
+        const unsigned long long hit = __ballot(tok >= q0 && tok < q0 + lq);
+        if (hit) {
+            parts = parts_of(a, __shfl(lk, __builtin_ctzll(hit), 64));
+            break;
+        }
+    }
+    if (parts == 1) return;                              // finished already, or in no document
     float m = -3.0e38f;
-    for (int s = 0; s < a.n_splits; ++s) m = __builtin_fmaxf(m, ws_stat<D>(a, s, row)[0]);
+    for (int s = lane; s < parts; s += 64) m = __builtin_fmaxf(m, ws_stat<D>(a, s, row)[0]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
     float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.n_splits; ++s) {
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
         const float2 st = *reinterpret_cast<const float2*>(ws_stat<D>(a, s, row));
         const float w = __builtin_amdgcn_exp2f(st.x - m);
         const float* p = ws_row<D>(a, s, row);
@@ -637,38 +690,49 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
     else dst[lane] = f2bf(o0 * inv);
 }
 
-// Rows per workgroup and key splits of a launch, from what the host knows: totals, the number of documents and the
-// caller's bounds on a document's lengths (hints: they size the grid, the kernels read the lengths themselves).
+// How a call is launched, from what the host knows: totals, the number of documents and the caller's bounds on a
+// document's lengths (hints: the kernels read the lengths themselves).
 struct Plan {
-    int waves, row_blocks, splits;
+    int waves;               // per workgroup: 32 query rows each
+    bool split;              // the split kernel (a document's keys in up to max_splits parts of about `chunk` tiles)
+    int row_blocks, chunk, max_splits;
 };
 
-Plan plan_of(long total_q, int docs, int kv_heads, int group, long max_q, long max_k) {
+Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, long max_q, long max_k) {
     Plan p;
+    const long cus = ovd_device_cus();
     max_q = max_q < 1 ? 1 : (max_q > total_q ? total_q : max_q);
+    max_k = max_k < 1 ? 1 : (max_k > total_k ? (total_k < 1 ? 1 : total_k) : max_k);
     const long rows = max_q * group;
-    // 256-row workgroups when they fill the chip, 128 rows otherwise
-    p.waves = rows <= 32 ? 1 : (total_q * group / 256 * kv_heads >= ovd_device_cus() ? 8 : 4);
+    // 256-row workgroups when they fill the chip, 128 rows otherwise, one wave when 32 rows hold a document's queries
+    p.waves = rows <= 32 ? 1 : (total_q * group / 256 * kv_heads >= cus ? 8 : 4);
     const long per = 32L * p.waves;
     p.row_blocks = (int)(total_q * group / per + docs);        // >= the sum of ceil(Lq group / per) over the documents
-    p.splits = 1;
-    const long wgs = (long)p.row_blocks * kv_heads;
-    if (p.waves == 1 && wgs < 2L * ovd_device_cus()) {
-        const long want = (2L * ovd_device_cus() + wgs - 1) / (wgs > 0 ? wgs : 1);
-        const long most = (max_k + 4 * BKV - 1) / (4 * BKV);       // at least 4 tiles each
-        p.splits = (int)(want < most ? want : most);
-        if (p.splits > 64) p.splits = 64;
-        if (p.splits < 1) p.splits = 1;
+    p.split = p.waves == 1 || (p.waves == 4 && (long)p.row_blocks * kv_heads <= cus);
+    p.chunk = 1 << 30;
+    p.max_splits = 1;
+    if (p.split) {
+        // parts of total / (8 workgroups per CU) tiles, at least 4 (a workgroup's start costs about as much as two)
+        const long most = (max_k + BKV - 1) / BKV;
+        long tiles = p.waves == 1 ? total_k / BKV + docs : most * p.row_blocks;
+        if (tiles > most * p.row_blocks) tiles = most * p.row_blocks;
+        long chunk = (tiles * kv_heads + 8 * cus - 1) / (8 * cus);
+        if (chunk < 4) chunk = 4;
+        p.chunk = (int)chunk;
+        p.max_splits = (int)((most + chunk - 1) / chunk);
+        if (p.max_splits > 256) p.max_splits = 256;
+        p.row_blocks = (int)(tiles / chunk + p.row_blocks);     // work items, were every length at its bound
     }
     return p;
 }
 
 }  // namespace
 
-long ovd_impl_attn_packed_workspace(long total_q, int docs, int q_heads, int kv_heads, int D, long max_q, long max_k) {
-    if (total_q <= 0 || docs <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
-    const Plan p = plan_of(total_q, docs, kv_heads, q_heads / kv_heads, max_q, max_k);
-    return p.splits > 1 ? (long)p.splits * total_q * q_heads * (D + 2) * (long)sizeof(float) : 0;
+long ovd_impl_attn_packed_workspace(long total_q, long total_k, int docs, int q_heads, int kv_heads, int D, long max_q,
+                                    long max_k) {
+    if (total_q <= 0 || docs <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads) return 0;
+    const Plan p = plan_of(total_q, total_k, docs, kv_heads, q_heads / kv_heads, max_q, max_k);
+    return p.max_splits > 1 ? (long)p.max_splits * total_q * q_heads * (D + 2) * (long)sizeof(float) : 0;
 }
 
 int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, long total_q, long total_k,
@@ -693,7 +757,6 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     OVD_REQUIRE(prefix == nullptr || causal, "attn_packed: a prefix goes with the causal mask");
     OVD_REQUIRE(max_q >= 0 && max_k >= 0, "attn_packed: negative length bound");
     if (total_q == 0) return 0;
-    if (max_k > total_k) max_k = total_k;       // the workspace was sized for the caller's bound: never more splits
     Args a;
     a.q = q; a.k = k; a.v = v; a.o = out;
     a.q_ld = q_ld; a.k_ld = k_ld; a.v_ld = v_ld; a.o_ld = o_ld;
@@ -703,38 +766,43 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.cap_in = softcap > 0.f ? 2.f * a.scale_log2 / softcap : 0.f;
     a.cap_out = softcap * 1.4426950408889634f;
-    Plan p = plan_of(total_q, docs, kv_heads, a.group, max_q, max_k);
-    if (p.splits > 1 && (workspace == nullptr ||
-                         (long)p.splits * total_q * q_heads * (D + 2) * (long)sizeof(float) > workspace_bytes))
-        p.splits = 1;
+    const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, max_q, max_k);
+    // no (or too small a) workspace: every document in one part
+    const long part_bytes = total_q * q_heads * (D + 2) * (long)sizeof(float);
+    const long room = workspace == nullptr ? 0 : workspace_bytes / part_bytes;
+    a.max_splits = room < p.max_splits ? (room < 2 ? 1 : (int)room) : p.max_splits;
+    a.chunk = p.chunk;
     a.row_blocks = p.row_blocks;
-    a.n_splits = p.splits;
     a.ws = (float*)workspace;
-    const long grid = (long)p.row_blocks * kv_heads * p.splits;
+    OVD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "attn_packed: the workspace must be 16-byte aligned");
+    const long grid = (long)p.row_blocks * kv_heads;
     OVD_REQUIRE(grid < (1L << 31), "attn_packed: grid too large");
     const size_t lds = 4 * BKV * D * 2;
-#define PACKED(DD, NW, CAP)                                                                                     \
+#define PACKED(KERNEL, NW)                                                                                      \
     {                                                                                                           \
         static OvdLdsLimit lim;                                                                                 \
-        if (!lim.ensure(reinterpret_cast<const void*>(&attn_packed_kernel<DD, NW, CAP>), lds))                  \
+        if (!lim.ensure(reinterpret_cast<const void*>(&KERNEL), lds))                                           \
             OVD_FAIL("attn_packed: cannot reserve %zu bytes of LDS", lds);                                      \
-        hipLaunchKernelGGL((attn_packed_kernel<DD, NW, CAP>), dim3((unsigned)grid), dim3(64 * NW), lds, st, a); \
+        hipLaunchKernelGGL((KERNEL), dim3((unsigned)grid), dim3(64 * NW), lds, st, a);                          \
     }
-#define PACKED_D(DD)                                                    \
-    {                                                                   \
-        if (p.waves == 1) {                                             \
-            if (softcap > 0.f) PACKED(DD, 1, true) else PACKED(DD, 1, false) \
-        } else if (p.waves == 8) {                                      \
-            if (softcap > 0.f) PACKED(DD, 8, true) else PACKED(DD, 8, false) \
-        } else {                                                        \
-            if (softcap > 0.f) PACKED(DD, 4, true) else PACKED(DD, 4, false) \
-        }                                                               \
+#define PACKED_KIND(DD, CAP)                                                                                    \
+    {                                                                                                           \
+        if (p.waves == 8) PACKED(PK(attn_packed_kernel, DD, 8, CAP), 8)                                         \
+        else if (!p.split) PACKED(PK(attn_packed_kernel, DD, 4, CAP), 4)                                        \
+        else if (p.waves == 4) PACKED(PK(attn_packed_split_kernel, DD, 4, CAP), 4)                              \
+        else PACKED(PK(attn_packed_split_kernel, DD, 1, CAP), 1)                                                \
     }
-    if (D == 128) PACKED_D(128) else PACKED_D(64)
-#undef PACKED_D
+#define PK(K, DD, NW, CAP) (K<DD, NW, CAP>)
+    if (D == 128) {
+        if (softcap > 0.f) PACKED_KIND(128, true) else PACKED_KIND(128, false)
+    } else {
+        if (softcap > 0.f) PACKED_KIND(64, true) else PACKED_KIND(64, false)
+    }
+#undef PK
+#undef PACKED_KIND
 #undef PACKED
     OVD_CHECK_LAUNCH("attn_packed");
-    if (p.splits > 1) {
+    if (p.split && a.max_splits > 1) {
         const long rows = total_q * q_heads;
         const dim3 jg((unsigned)((rows + 3) / 4)), jb(256);
         if (D == 128) hipLaunchKernelGGL(attn_packed_join_kernel<128>, jg, jb, 0, st, a);

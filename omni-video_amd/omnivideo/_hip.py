@@ -55,7 +55,7 @@ SIGNATURES = {
     "ovd_linear_mxfp4_workspace_bytes": [_i, _i],
     "ovd_linear_mxfp4": [_p, _i, _l, _p, _p, _p, _p, _l, _p, _p, _l, _i, _i, _i, _i, _p],
     "ovd_rope_positions": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _l, _l, _i, _i, _i, _i, _p],
-    "ovd_attn_packed_workspace_bytes": [_l, _i, _i, _i, _i, _l, _l],
+    "ovd_attn_packed_workspace_bytes": [_l, _l, _i, _i, _i, _i, _l, _l],
     "ovd_attn_packed_fwd_bf16": [_p, _p, _p, _p, _l, _l, _p, _p, _i, _l, _l, _i, _i, _i, _l, _l, _l, _l, _i, _p, _f, _f, _p,
                                  _l, _p],
     "ovd_resize_coeffs": [_i, _i, _p, _p, _i],
@@ -833,10 +833,10 @@ def rope_positions(x, pos, freq, axis, out, interleaved=True, inverse=False):
     return out
 
 
-def attn_packed_workspace_bytes(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k):
+def attn_packed_workspace_bytes(total_q, total_k, docs, q_heads, kv_heads, head_dim, max_q, max_k):
     """Bytes with which attn_packed splits long documents over workgroups when there are few query rows (0: no use).
     Depends on the current device's compute units."""
-    return int(lib().ovd_attn_packed_workspace_bytes(total_q, docs, q_heads, kv_heads, head_dim, max_q, max_k))
+    return int(lib().ovd_attn_packed_workspace_bytes(total_q, total_k, docs, q_heads, kv_heads, head_dim, max_q, max_k))
 
 
 def attn_packed(q, k, v, cu_q, cu_k, out, max_q, max_k, causal=False, prefix=None, softmax_scale=None, softcap=0.0,

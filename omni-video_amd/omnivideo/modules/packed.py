@@ -99,8 +99,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=Fa
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if workspace is None and q.is_cuda and Tq:
-        with torch.cuda.device(q.device):
-            n = H.attn_packed_workspace_bytes(Tq, cu_q.numel() - 1, Nq, k.shape[1], D, min(max_q, Tq), min(max_k, k.shape[0]))
+        n = H.attn_packed_workspace_bytes(Tq, k.shape[0], cu_q.numel() - 1, Nq, k.shape[1], D, max_q, max_k)
         if n > 0:
             workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
     return H.attn_packed(q, k, v, cu_q, cu_k, out, max_q, max_k, causal, prefix, softmax_scale, softcap, workspace)

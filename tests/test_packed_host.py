@@ -114,7 +114,8 @@ def test_c_entries_refuse_before_any_launch():
 
 
 def test_workspace_sizes(monkeypatch):
-    assert H.attn_packed_workspace_bytes(0, 1, 8, 8, 128, 1, 1) == 0
-    assert H.attn_packed_workspace_bytes(20280, 4, 40, 40, 128, 9000, 9000) == 0          # enough rows: not split
-    n = H.attn_packed_workspace_bytes(8, 8, 40, 8, 128, 1, 32760)
+    assert H.attn_packed_workspace_bytes(0, 5, 1, 8, 8, 128, 1, 1) == 0
+    assert H.attn_packed_workspace_bytes(20280, 20280, 4, 40, 40, 128, 9000, 9000) == 0          # enough rows: not split
+    assert H.attn_packed_workspace_bytes(8, 800, 8, 40, 8, 128, 1, 100) == 0                     # short documents: neither
+    n = H.attn_packed_workspace_bytes(8, 80000, 8, 40, 8, 128, 1, 32760)
     assert n > 0 and n % (8 * 40 * 130 * 4) == 0
