@@ -645,13 +645,15 @@ __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_split_ke
 #endif
 }
 
-// out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts, in their order; one wave per (token, head)
+// out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts; one workgroup per (token, head), its waves take
+// the parts in turn and meet in a fixed order
 template <int D>
 __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
-    const int lane = threadIdx.x & 63;
+    __shared__ float2 acc[4][64];
+    __shared__ float den[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int heads = a.kv_heads * a.group;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (long)a.total_q * heads) return;
+    const long row = blockIdx.x;
     const int tok = (int)(row / heads), head = (int)(row % heads);
     int parts = 1;
     for (int d0 = 0; d0 < a.docs; d0 += 64) {            // the token's document
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
     for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
     float l = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
+    for (int s = wave; s < parts; s += 4) {
         const float2 st = *reinterpret_cast<const float2*>(ws_stat<D>(a, s, row));
         const float w = __builtin_amdgcn_exp2f(st.x - m);
         const float* p = ws_row<D>(a, s, row);
@@ -684,6 +686,13 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(Args a) {
             o0 = fmaf(p[lane], w, o0);
         }
     }
+    acc[wave][lane] = make_float2(o0, o1);
+    if (lane == 0) den[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    l = (den[0] + den[1]) + (den[2] + den[3]);
+    o0 = (acc[0][lane].x + acc[1][lane].x) + (acc[2][lane].x + acc[3][lane].x);
+    o1 = (acc[0][lane].y + acc[1][lane].y) + (acc[2][lane].y + acc[3][lane].y);
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     bf16_t* dst = a.o + (long)tok * a.o_ld + (long)head * D;
     if constexpr (D == 128) reinterpret_cast<uint32_t*>(dst)[lane] = pack_bf2(o0 * inv, o1 * inv);
@@ -698,7 +707,7 @@ struct Plan {
     int row_blocks, chunk, max_splits;
 };
 
-Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, long max_q, long max_k) {
+Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, int D, long max_q, long max_k) {
     Plan p;
     const long cus = ovd_device_cus();
     max_q = max_q < 1 ? 1 : (max_q > total_q ? total_q : max_q);
@@ -712,12 +721,26 @@ Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, long
     p.chunk = 1 << 30;
     p.max_splits = 1;
     if (p.split) {
-        // parts of total / (8 workgroups per CU) tiles, at least 4 (a workgroup's start costs about as much as two)
+        // All parts have about the same number of tiles, `chunk`, and `slots` workgroups run at a time.  R rounds leave
+        // R slots - (one partly filled part per row block) parts for the tiles; a workgroup's start costs about as much
+        // as 4 tiles.  The number of rounds that this puts first (8 tokens against 1 to 32760 keys, 8 key heads: one
+        // round of 23 tiles 69 us, four rounds of 5 tiles 88 us).
         const long most = (max_k + BKV - 1) / BKV;
         long tiles = p.waves == 1 ? total_k / BKV + docs : most * p.row_blocks;
         if (tiles > most * p.row_blocks) tiles = most * p.row_blocks;
-        long chunk = (tiles * kv_heads + 8 * cus - 1) / (8 * cus);
-        if (chunk < 4) chunk = 4;
+        const long slots = (D == 64 && p.waves == 1 ? 4 : 2) * cus, blocks = (long)p.row_blocks * kv_heads;
+        long chunk = most, best = -1;
+        for (long r = 1; r <= 8; ++r) {
+            if (r * slots <= blocks) continue;
+            long c = (tiles * kv_heads + (r * slots - blocks) - 1) / (r * slots - blocks);
+            c = c < 4 ? 4 : (c > most ? most : c);
+            const long cost = r * (c + 4);
+            if (best < 0 || cost < best) {
+                best = cost;
+                chunk = c;
+            }
+        }
+        if (chunk < 1) chunk = 1;
         p.chunk = (int)chunk;
         p.max_splits = (int)((most + chunk - 1) / chunk);
         if (p.max_splits > 256) p.max_splits = 256;
@@ -731,7 +754,7 @@ Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, long
 long ovd_impl_attn_packed_workspace(long total_q, long total_k, int docs, int q_heads, int kv_heads, int D, long max_q,
                                     long max_k) {
     if (total_q <= 0 || docs <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads) return 0;
-    const Plan p = plan_of(total_q, total_k, docs, kv_heads, q_heads / kv_heads, max_q, max_k);
+    const Plan p = plan_of(total_q, total_k, docs, kv_heads, q_heads / kv_heads, D, max_q, max_k);
     return p.max_splits > 1 ? (long)p.max_splits * total_q * q_heads * (D + 2) * (long)sizeof(float) : 0;
 }
 
@@ -766,7 +789,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.cap_in = softcap > 0.f ? 2.f * a.scale_log2 / softcap : 0.f;
     a.cap_out = softcap * 1.4426950408889634f;
-    const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, max_q, max_k);
+    const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, D, max_q, max_k);
     // no (or too small a) workspace: every document in one part
     const long part_bytes = total_q * q_heads * (D + 2) * (long)sizeof(float);
     const long room = workspace == nullptr ? 0 : workspace_bytes / part_bytes;
@@ -804,7 +827,8 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     OVD_CHECK_LAUNCH("attn_packed");
     if (p.split && a.max_splits > 1) {
         const long rows = total_q * q_heads;
-        const dim3 jg((unsigned)((rows + 3) / 4)), jb(256);
+        OVD_REQUIRE(rows < (1L << 31), "attn_packed: grid too large");
+        const dim3 jg((unsigned)rows), jb(256);
         if (D == 128) hipLaunchKernelGGL(attn_packed_join_kernel<128>, jg, jb, 0, st, a);
         else hipLaunchKernelGGL(attn_packed_join_kernel<64>, jg, jb, 0, st, a);
         OVD_CHECK_LAUNCH("attn_packed join");

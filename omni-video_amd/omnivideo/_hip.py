@@ -808,26 +808,30 @@ def linear_mxfp4(x, w, out, bias=None, epilogue=EPI_BF16, gate=None):
 
 def _packed_heads(name, t):
     """token stride of [T, N, D] with dense heads"""
-    if t.dim() != 3 or t.shape[1] < 1 or (t.shape[2] > 1 and t.stride(2) != 1) \
-            or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    if t.dim() != 3:
         raise ValueError(f"{name}: tensors must be [tokens, heads, head_dim] with dense (heads, head_dim)")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    T, N, D = t.shape
+    st, sn, sd = t.stride()
+    if N < 1 or (sd != 1 and D > 1) or (sn != D and N > 1):
+        raise ValueError(f"{name}: tensors must be [tokens, heads, head_dim] with dense (heads, head_dim)")
+    return st if T > 1 else N * D
 
 
 def rope_positions(x, pos, freq, axis, out, interleaved=True, inverse=False):
     """x, out [T, N, D] bf16 or fp32, pos [T, A] int32 or fp32, freq fp64 [D / 2] (revolutions), axis int32 [D / 2]."""
     ldx, ldo = _packed_heads("rope", x), _packed_heads("rope", out)
     T, N, D = x.shape
-    if out.shape != x.shape or out.dtype != x.dtype or x.dtype not in (BF16, F32):
+    xt, pt = x.dtype, pos.dtype
+    if out.shape != x.shape or out.dtype != xt or xt not in (BF16, F32):
         raise ValueError("rope: x and out must be bf16 or fp32 tensors of one shape and type")
-    if pos.dim() != 2 or pos.shape[0] != T or pos.dtype not in (torch.int32, F32) or not pos.is_contiguous():
-        raise ValueError(f"rope: positions must be contiguous int32 or fp32 [{T}, axes], got {tuple(pos.shape)} {pos.dtype}")
+    if pos.dim() != 2 or pos.shape[0] != T or pt not in (torch.int32, F32) or not pos.is_contiguous():
+        raise ValueError(f"rope: positions must be contiguous int32 or fp32 [{T}, axes], got {tuple(pos.shape)} {pt}")
     if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.numel() != D // 2 or axis.numel() != D // 2 \
             or not freq.is_contiguous() or not axis.is_contiguous():
         raise ValueError(f"rope: the frequency table is not one of {D // 2} pairs")
     dev = _one_device(x, pos, freq, axis, out)
     if T:
-        _call_on(dev, "ovd_rope_positions", x.data_ptr(), int(x.dtype == F32), ldx, pos.data_ptr(), int(pos.dtype == F32),
+        _call_on(dev, "ovd_rope_positions", x.data_ptr(), int(xt == F32), ldx, pos.data_ptr(), int(pt == F32),
                  pos.shape[1], freq.data_ptr(), axis.data_ptr(), out.data_ptr(), ldo, T, N, D, int(interleaved),
                  int(inverse))
     return out

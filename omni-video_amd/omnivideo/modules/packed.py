@@ -12,8 +12,9 @@ BF16, F32 = torch.bfloat16, torch.float32
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise NotImplementedError("packed operators: inference only; call under torch.no_grad() or detach the inputs")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("packed operators: inference only; call under torch.no_grad() or detach the inputs")
 
 
 class RopePlan:
@@ -73,8 +74,10 @@ def packed_rope(x, positions, plan, out=None, inverse=False):
     if x.dim() != 3 or x.shape[2] != plan.head_dim:
         raise ValueError(f"packed_rope: x must be [tokens, heads, {plan.head_dim}], got {tuple(x.shape)}")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    return H.rope_positions(x, positions.contiguous(), plan.freq, plan.axis, out, plan.interleaved, inverse)
+        out = x.new_empty(x.shape)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    return H.rope_positions(x, positions, plan.freq, plan.axis, out, plan.interleaved, inverse)
 
 
 def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=False, prefix=None, softcap=0.0,
@@ -97,7 +100,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=Fa
     max_q = Tq if max_q is None else int(max_q)
     max_k = k.shape[0] if max_k is None else int(max_k)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     if workspace is None and q.is_cuda and Tq:
         n = H.attn_packed_workspace_bytes(Tq, k.shape[0], cu_q.numel() - 1, Nq, k.shape[1], D, max_q, max_k)
         if n > 0:
