@@ -223,7 +223,7 @@ def test_attention_large_scores(P):
     Lq, Lk = [70, 3], [500, 400]
     q, k, v = inputs(Lq, Lk, 2, 2, 128, 9, 4.0)
     k[450] = q[0, 0:2] * 3
-    for cap in (0.0, 50.0):
+    for cap in (0.0, 50.0, 5.0, 300.0, 0.01, 1e6):       # scores past the cap, around half of it, far below it
         want, bound = ref_attention(q, k, v, Lq, Lk, False, None, cap, 128 ** -0.5)
         check(P.packed_attention(q, k, v, cu(Lq), cu(Lk), softcap=cap), want, bound)
 
