@@ -21,7 +21,7 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
-enum Epi { EPI_BF16 = 0, EPI_BF16_GELU = 1, EPI_F32 = 2, EPI_RESID = 3 };
+enum Epi { EPI_BF16 = 0, EPI_BF16_GELU = 1, EPI_F32 = 2, EPI_RESID = 3, EPI_MX_GELU = 4 };
 
 constexpr int KG = 256;                 // k-group: four MFMA k-steps, one scale dword per lane
 constexpr int FRAG = 1024;              // bytes of a 32-row x 64-k fragment
@@ -203,6 +203,59 @@ __device__ __forceinline__ void store4(const Out& o, long m, int n, float (&y)[4
     }
 }
 
+// EPI_MX_GELU: the 32 x 32 block of outputs that a wave holds in `acc` (register 4 g + j of lane l: row l & 31, column
+// 8 g + 4 (l >> 5) + j) through bias and GELU and, still in fp32, into one MX block per row of the next product's operand:
+// a row's 32 values lie in two lanes, so its largest magnitude is 15 maxima and one exchange, and each lane ends up with
+// the whole 16 bytes of codes.  o.out: the codes, o.gate: the scales (as addresses), N columns, out_groups k-groups a row
+// block.  Columns past N are written as zeros: they are the padding of that operand.
+__device__ __forceinline__ void store_mx(const Out& o, const f32x16& acc, long rb, int nb, long m, int M, int N, int out_groups,
+                                         int lane) {
+    const int h = lane >> 5;
+    float y[16];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int n = nb * 32 + 8 * g + 4 * h;
+        uint2 b = make_uint2(0, 0);
+        if (o.bias && n < N) b = *reinterpret_cast<const uint2*>(o.bias + n);
+        y[4 * g] = acc[4 * g] + bf2f(b.x & 0xffff);
+        y[4 * g + 1] = acc[4 * g + 1] + bf2f(b.x >> 16);
+        y[4 * g + 2] = acc[4 * g + 2] + bf2f(b.y & 0xffff);
+        y[4 * g + 3] = acc[4 * g + 3] + bf2f(b.y >> 16);
+    }
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        y[i] = nb * 32 < N ? gelu_tanh_f(y[i]) : 0.f;
+        mx = umax(mx, __float_as_uint(y[i]) & 0x7fffffffu);
+    }
+    const auto ex = __builtin_amdgcn_permlane32_swap(mx, mx, false, false);
+    const uint32_t s = scale_byte(umax(ex[0], ex[1]));
+    const float inv = inv_scale(s);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] *= inv;
+    uint32_t w[2];                       // this lane's codes: 4 g + j ascending, 16 bits per g
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        uint32_t u = 0;
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q], y[8 * q + 1], 1.0f, 0);
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 2], y[8 * q + 3], 1.0f, 1);
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 4], y[8 * q + 5], 1.0f, 2);
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 6], y[8 * q + 7], 1.0f, 3);
+        w[q] = u;
+    }
+    // word g of the block = columns 8 g .. 8 g + 7: 16 bits from the lower lane, 16 from the upper
+    const auto e0 = __builtin_amdgcn_permlane32_swap(w[0], w[0], false, false);
+    const auto e1 = __builtin_amdgcn_permlane32_swap(w[1], w[1], false, false);
+    if (h == 0 && m < M) {
+        uint8_t* data = reinterpret_cast<uint8_t*>(o.out) + ((rb * out_groups + (nb >> 3)) * 4 + ((nb >> 1) & 3)) * FRAG;
+        *reinterpret_cast<uint4*>(data + ((nb & 1) * 32 + (lane & 31)) * 16) =
+            make_uint4((e0[0] & 0xffffu) | (e0[1] << 16), (e0[0] >> 16) | (e0[1] & 0xffff0000u),
+                       (e1[0] & 0xffffu) | (e1[1] << 16), (e1[0] >> 16) | (e1[1] & 0xffff0000u));
+        uint8_t* scale = reinterpret_cast<uint8_t*>(const_cast<float*>(o.gate)) + (rb * out_groups + (nb >> 3)) * GRP_SCALE;
+        scale[((nb & 1) * 32 + (lane & 31)) * 4 + ((nb >> 1) & 3)] = (uint8_t)s;
+    }
+}
+
 // one 32-row x 256-k group of an operand in registers
 struct Group {
     uint4 f[4];
@@ -283,6 +336,29 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
                 part[(wave * Q + (i * NT + j) * 4 + g) * 64 + lane] =
                     make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
     __syncthreads();
+    if constexpr (EPI == EPI_MX_GELU) {          // an MX block needs all 32 columns of a row: one wave per 32 x 32 block
+        if (wave >= MT * NT) return;
+        f32x16 t;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float4 p = part[(k * Q + wave * 4 + g) * 64 + lane];
+                y.x += p.x;
+                y.y += p.y;
+                y.z += p.z;
+                y.w += p.w;
+            }
+            t[4 * g] = y.x;
+            t[4 * g + 1] = y.y;
+            t[4 * g + 2] = y.z;
+            t[4 * g + 3] = y.w;
+        }
+        const long rb = rb0 + wave / NT;
+        store_mx(o, t, rb, (int)(nb0 + wave % NT), rb * 32 + (lane & 31), A.rows, W.rows, (W.rows + KG - 1) / KG, lane);
+        return;
+    }
     for (int q = wave; q < Q; q += 8) {
         float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -296,7 +372,9 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
         const int g = q & 3, j = (q >> 2) % NT, i = (q >> 2) / NT;
         const long m = (rb0 + i) * 32 + (lane & 31);
         const int n = (int)(nb0 + j) * 32 + 8 * g + 4 * (lane >> 5);
-        if (m < A.rows && n < W.rows) store4<EPI>(o, m, n, y);
+        if constexpr (EPI != EPI_MX_GELU) {
+            if (m < A.rows && n < W.rows) store4<EPI>(o, m, n, y);
+        }
     }
 }
 
@@ -555,6 +633,19 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
     // chunk c of row r at c ^ (r & 15)) so that 32 lanes store one 512-byte row segment.
     constexpr bool NARROW = EPI == EPI_BF16 || EPI == EPI_BF16_GELU;
     const int fr = lane & 31, fh = lane >> 5;
+    if constexpr (EPI == EPI_MX_GELU) {          // a tile's 256 columns are one k-group of the next operand
+        const int out_groups = (W.rows + KG - 1) / KG;
+#pragma unroll
+        for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+                for (int nh = 0; nh < 2; ++nh) {
+                    const long rb = tm * 8 + mh * 4 + wr * 2 + mb;
+                    store_mx(o, acc[nh][mh * 2 + mb], rb, tn * 8 + nh * 4 + wc, rb * 32 + fr, A.rows, W.rows, out_groups, lane);
+                }
+        return;
+    }
     const bool staged = NARROW && wide;
 #pragma unroll
     for (int mh = 0; mh < 2; ++mh) {
@@ -573,7 +664,9 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
                     const f32x16& a16 = acc[nh][mh * 2 + mb];
                     float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
                     if (!staged) {
-                        if (n < W.rows) store4<EPI>(o, m, n, y);
+                        if constexpr (EPI != EPI_MX_GELU) {
+                            if (n < W.rows) store4<EPI>(o, m, n, y);
+                        }
                         continue;
                     }
                     if (o.bias) {
@@ -687,13 +780,19 @@ static int check_out(int M, int N, int K, int epilogue, const void* out, long ld
                      const void* w_data, const void* w_scale) {
     OVD_REQUIRE(M >= 0 && N > 0 && N % 4 == 0 && K > 0 && K % 32 == 0,
                 "gemm_mxfp4: M=%d N=%d K=%d not supported: N %% 4, K %% 32", M, N, K);
-    OVD_REQUIRE(epilogue >= EPI_BF16 && epilogue <= EPI_RESID, "gemm_mxfp4: unknown epilogue %d", epilogue);
+    OVD_REQUIRE(epilogue >= EPI_BF16 && epilogue <= EPI_MX_GELU, "gemm_mxfp4: unknown epilogue %d", epilogue);
+    OVD_REQUIRE(reinterpret_cast<uintptr_t>(w_data) % 16 == 0 && reinterpret_cast<uintptr_t>(w_scale) % 4 == 0,
+                "gemm_mxfp4: operands must be 16-byte aligned");
+    if (epilogue == EPI_MX_GELU) {
+        OVD_REQUIRE(N % 32 == 0 && gate != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(gate) % 4 == 0 && reinterpret_cast<uintptr_t>(bias) % 8 == 0,
+                    "gemm_mxfp4: an MXFP4 output needs N %% 32 == 0 (N=%d), codes and scales", N);
+        return 0;
+    }
     OVD_REQUIRE(gate == nullptr || epilogue == EPI_RESID, "gemm_mxfp4: a gate goes with the residual epilogue");
     OVD_REQUIRE(ldo >= N && ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (epilogue <= EPI_BF16_GELU ? 8 : 16) == 0 &&
                     reinterpret_cast<uintptr_t>(bias) % 8 == 0 && reinterpret_cast<uintptr_t>(gate) % 16 == 0,
                 "gemm_mxfp4: out rows, bias and gate must be aligned to 4 values (ldo=%ld)", ldo);
-    OVD_REQUIRE(reinterpret_cast<uintptr_t>(w_data) % 16 == 0 && reinterpret_cast<uintptr_t>(w_scale) % 4 == 0,
-                "gemm_mxfp4: operands must be 16-byte aligned");
     return 0;
 }
 
@@ -702,6 +801,7 @@ int ovd_impl_linear_mxfp4(const void* x, int x_is_f32, long ldx, const uint8_t* 
                           int M, int N, int K, int epilogue, hipStream_t st) {
     if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
     if (M == 0) return 0;
+    OVD_REQUIRE(epilogue != EPI_MX_GELU || !few_rows(M, K), "linear_mxfp4: an MXFP4 output takes a quantised x (ovd_gemm_mxfp4)");
     if (!few_rows(M, K)) {
         const long nd = ovd_impl_mxfp4_data_bytes(M, K);
         OVD_REQUIRE(workspace != nullptr && workspace_bytes >= ovd_impl_linear_mxfp4_workspace(M, K),
@@ -751,7 +851,8 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
             OVD_FAIL("gemm_mxfp4: cannot reserve %zu bytes of LDS", lds);                                      \
         const int ty = ceil_div(M, 32 * MT);                                                                   \
         OVD_REQUIRE(ty <= 65535, "gemm_mxfp4: grid too large");                                                \
-        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(N, 32 * NT), ty), dim3(512),   \
+        const int cols = E == EPI_MX_GELU ? ceil_div(N, KG) * KG : N;                                          \
+        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(cols, 32 * NT), ty), dim3(512), \
                            lds, st, A, W, o, groups);                                                          \
     }
 #define BIG(E)                                                                                                 \
@@ -768,7 +869,7 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
     const bool big = groups >= 2 && (long)tiles_m * tiles_n >= cus / 2;
     const int wide = (ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) ? 1 : 0;
 #define GEMM_CASE(E) case E: if (big) BIG(E) else if (M <= 32) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
-    switch (epilogue) { GEMM_CASE(EPI_BF16) GEMM_CASE(EPI_BF16_GELU) GEMM_CASE(EPI_F32) GEMM_CASE(EPI_RESID) }
+    switch (epilogue) { GEMM_CASE(EPI_BF16) GEMM_CASE(EPI_BF16_GELU) GEMM_CASE(EPI_F32) GEMM_CASE(EPI_RESID) GEMM_CASE(EPI_MX_GELU) }
 #undef GEMM_CASE
 #undef BIG
 #undef DIRECT

@@ -779,6 +779,24 @@ def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
     return out
 
 
+EPI_MXFP4_GELU = 4
+
+
+def gemm_mxfp4_gelu(a, w, out, bias=None):
+    """out (MXFP4 matrix [M, N]) = quantised gelu(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]."""
+    M, N, K = a.rows, w.rows, a.cols
+    if w.cols != K or out.rows != M or out.cols != N:
+        raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}] out[{out.rows},{out.cols}]")
+    if bias is not None and (bias.numel() != N or not bias.is_contiguous() or bias.dtype != BF16):
+        raise ValueError(f"gemm_mxfp4: bias must be a contiguous bf16 row of length {N}")
+    dev = _one_device(a.buf, w.buf, out.buf, bias)
+    (ad, asc), (wd, wsc), (od, osc) = a.pointers(), w.pointers(), out.pointers()
+    if M:
+        _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), od, N, osc, M, N, K,
+                 EPI_MXFP4_GELU)
+    return out
+
+
 MXFP4_FEW_ROWS = 8           # up to this many rows linear_mxfp4 quantises inside the product (one launch)
 
 

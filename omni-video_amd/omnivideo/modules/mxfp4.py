@@ -123,11 +123,14 @@ def mxfp4_quantize(x, out=None):
     return H.mxfp4_quant(x2, out)
 
 
-def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, residual=None, gate=None):
+def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, residual=None, gate=None,
+                 quantize_output=False):
     """act(x @ weight.T + bias) with both operands in MXFP4 and fp32 accumulation; one rounding, of the stored value.
     x: [..., K] bf16 or fp32 (quantised here), or an MXFP4Matrix; weight: MXFP4Matrix [N, K], N a multiple of 4;
     bias bf16 [N]; gelu: tanh-GELU (bf16 output).  Returns [..., N] in out_dtype (bf16 or fp32), written to `out` if given.
-    residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned."""
+    residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned.
+    quantize_output (with gelu, N a multiple of 32): the result as an MXFP4Matrix [M, N] (`out` if given), quantised from
+    fp32 in the product's own pass: the input of the next layer."""
     if not isinstance(weight, MXFP4Matrix):
         raise TypeError("mxfp4_linear: weight must be an MXFP4Matrix (mxfp4_quantize or MXFP4Matrix.from_ocp)")
     packed = isinstance(x, MXFP4Matrix)
@@ -136,6 +139,15 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
     lead = (x.rows,) if packed else x.shape[:-1]
     _no_grad(None if packed else x, bias, residual, gate)
     N = weight.rows
+    if quantize_output:
+        if not gelu or residual is not None or gate is not None:
+            raise ValueError("mxfp4_linear: quantize_output goes with gelu, and with neither residual nor gate")
+        a = x if packed else mxfp4_quantize(x)
+        if out is None:
+            out = MXFP4Matrix.empty(a.rows, N, weight.device)
+        elif not isinstance(out, MXFP4Matrix):
+            raise TypeError("mxfp4_linear: quantize_output writes an MXFP4Matrix")
+        return H.gemm_mxfp4_gelu(a, weight, out, bias)
     if residual is not None:
         if out is not None or gelu:
             raise ValueError("mxfp4_linear: residual goes with neither out nor gelu")

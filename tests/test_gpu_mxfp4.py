@@ -164,6 +164,46 @@ def test_linear_epilogues(X, M, N, K):
         close(x, x0.double() + wb * gd, bound_b * gd.abs(), F32)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 32, 64), (5, 96, 512), (33, 544, 288), (550, 1536, 1536), (300, 8960, 512),
+                                   (4127, 2080, 288), (8000, 1280, 512)])
+def test_linear_with_quantised_output(X, M, N, K):
+    """the output operand = the quantisation of the fp32 result: equal where the fp32 value is not within its own error
+    of a border of the rounding or of a power of two of the block's largest magnitude"""
+    a, w, prod, bound = operands(X, M, N, K, M + 7)
+    bias = randn((N,), 3, 0.1).to(BF16).cuda()
+    m = X.mxfp4_linear(a, w, bias, gelu=True, quantize_output=True)
+    assert isinstance(m, X.MXFP4Matrix) and m.shape == (M, N)
+    wb = prod + bias.double()
+    want = 0.5 * wb * (1 + torch.tanh(math.sqrt(2 / math.pi) * (wb + 0.044715 * wb ** 3)))
+    err = 1.13 * (bound + 2.0 ** -24 * (wb.abs() + bound)) + 2.0 ** -21 * wb.abs() + 1e-37
+    code, s, _ = ref_quant(want.cpu())
+    got_c, got_s = codes_of(m)
+    e = err.cpu().reshape(M, -1, 32)
+    top = want.cpu().abs().reshape(M, -1, 32)
+    lo, hi = (top - e).amax(2), (top + e).amax(2)
+    sure = torch.floor(torch.log2(lo.clamp(min=1e-300))) == torch.floor(torch.log2(hi))      # the block's scale
+    assert torch.equal(got_s[sure], s[sure])
+    assert float(sure.double().mean()) > 0.9 or N * M < 2000
+    assert ((got_s.int() - s.int()).abs() <= 1).all()
+    u = (want.cpu().abs().reshape(M, -1, 32) / torch.exp2(s.double() - 127)[..., None])
+    du = e / torch.exp2(s.double() - 127)[..., None]
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=F64)
+    clear = ((u[..., None] - borders).abs() > du[..., None]).all(-1) & sure[..., None]
+    mag = lambda c: (c & 7).reshape(M, -1, 32)
+    assert torch.equal(mag(got_c)[clear], mag(code)[clear])
+    sign_clear = clear & (mag(code) > 0)
+    assert torch.equal((got_c >> 3).reshape(M, -1, 32)[sign_clear], (code >> 3).reshape(M, -1, 32)[sign_clear])
+    # it is an operand of the next product, padding included
+    w2 = X.mxfp4_quantize(randn((64, N), 9, 1 / math.sqrt(N)).cuda())
+    A, W2 = m.dequantize(F32).double(), w2.dequantize(F32).double()
+    close(X.mxfp4_linear(m, w2, out_dtype=F32), A @ W2.t(), N * 2.0 ** -23 * (A.abs() @ W2.abs().t()), F32)
+    again = X.MXFP4Matrix.empty(M, N, "cuda")
+    again.buf.fill_(255)
+    assert X.mxfp4_linear(a, w, bias, gelu=True, quantize_output=True, out=again) is again
+    assert torch.equal(again.dequantize(F32), m.dequantize(F32))
+    close(X.mxfp4_linear(again, w2, out_dtype=F32), A @ W2.t(), N * 2.0 ** -23 * (A.abs() @ W2.abs().t()), F32)
+
+
 def test_linear_exact_on_small_integers(X):
     """whole numbers with scale 1 have exact sums: a wrong lane, block order, nibble order or scale byte shows as a
     wrong whole number.  Blocks get different scales, so each scale has to meet its own block."""

@@ -82,6 +82,12 @@ def test_python_entries_refuse():
         mxfp4_linear(a, w, gelu=True, residual=torch.zeros(4, 8))
     with pytest.raises(ValueError, match="gate"):
         mxfp4_linear(a, w, gate=torch.ones(8))
+    with pytest.raises(ValueError, match="quantize_output"):
+        mxfp4_linear(a, w, quantize_output=True)
+    with pytest.raises(TypeError, match="MXFP4Matrix"):
+        mxfp4_linear(a, w, gelu=True, quantize_output=True, out=torch.zeros(4, 8))
+    with pytest.raises(ValueError, match="no blocks"):
+        mxfp4_linear(a, w, gelu=True, quantize_output=True)
     with pytest.raises(ValueError, match="shape"):
         mxfp4_linear(a, w, out=torch.zeros(4, 9))
     with pytest.raises(ValueError, match="length"):
@@ -108,7 +114,10 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_mxfp4_dequant", p, p, p, 0, 16, 1, 32, None, why=b"alignment")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, None, 1, 6, 32, 0, None, why=b"not supported")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, None, 1, 8, 40, 0, None, why=b"not supported")
-    refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, None, 1, 8, 32, 4, None, why=b"epilogue")
+    refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, None, 1, 8, 32, 5, None, why=b"epilogue")
+    refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, p, 1, 8, 32, 4, None, why=b"MXFP4 output")
+    refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 32, None, 1, 32, 32, 4, None, why=b"MXFP4 output")
+    refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 32, p, None, 0, 2, 32, 32, 4, None, why=b"quantised x")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, p, 1, 8, 32, 0, None, why=b"gate")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 4, None, 1, 8, 32, 0, None, why=b"ldo")
     refused("ovd_gemm_mxfp4", p, p, p + 8, p, None, p, 8, None, 1, 8, 32, 0, None, why=b"16-byte")
