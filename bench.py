@@ -332,7 +332,7 @@ def main():
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--warmup", type=int, default=1)
     ap.add_argument("--workload", default="cfg2", choices=list(WORKLOADS))
-    ap.add_argument("--precision", choices=["bf16", "fp8"], default=None,
+    ap.add_argument("--precision", choices=["bf16", "fp8", "mxfp4"], default=None,
                     help="arithmetic of the large linear layers (default: the workload's; fp8 only for cfg5)")
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-cpu-baseline", action="store_true")
@@ -778,7 +778,7 @@ def main():
             "metric": "denoised frames/sec (whole node)", "value": round(value, 4) if sp_ok else None, "unit": "frames/s",
             "n_gpus": world, "steps": K, "warmup": W, "ms_per_step": round(ms_step, 3), "higher_is_better": True,
             "scaling": "strong" if (sp and n_groups == 1) else "weak", "vs_baseline": None,
-            "dtype": "bf16" if precision == "bf16" else "fp8 (e4m3 linear layers, int8 Q K^T in self-attention with bf16 P V, fp32 residual stream)",
+            "dtype": "bf16" if precision == "bf16" else f"{'fp8 (e4m3' if precision == 'fp8' else 'mxfp4 (e2m1'} linear layers, int8 Q K^T in self-attention with bf16 P V, fp32 residual stream)",
             "data": "synthetic",
             "config": {"workload": wl["desc"], "linear_precision": precision, "latent": list(wl["latent"]), "tokens": seq_len,
                        "context_len": wl["text_len"], "context_keys_read": k_len, "sampling_steps": wl["steps"], "guide_scale": 3.0,

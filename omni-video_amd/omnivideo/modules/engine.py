@@ -35,6 +35,7 @@ import torch
 import torch.distributed as dist
 
 from .. import _hip as H
+from .mxfp4 import MXFP4Matrix, mxfp4_quantize
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -151,7 +152,7 @@ def make_group_comm(group=None, kind=None):
     raise ValueError(f"OVD_SP_COMM / kind must be auto, rccl, host or peer, got {kind!r}")
 
 
-FP8_LINEARS = ("qkv", "o", "cq", "co", "f0", "f2")
+FP8_LINEARS = ("qkv", "o", "cq", "co", "f0", "f2")      # the layers of a block that the reduced-precision modes serve
 
 
 def planned_bytes(cfg, grid, seq_len, nb, text_len, sp=1, precision="bf16", attention=None, attn_workspace=0):
@@ -162,13 +163,16 @@ def planned_bytes(cfg, grid, seq_len, nb, text_len, sp=1, precision="bf16", atte
     shape, which depends on the device), "total"}.  cfg: the WanModel configuration (dim, ffn_dim, num_heads,
     num_layers, text_dim, freq_dim, in_dim, out_dim, patch_size)."""
     C, F, N, nl = cfg["dim"], cfg["ffn_dim"], cfg["num_heads"], cfg["num_layers"]
-    attention = attention or ("int8" if precision == "fp8" else "bf16")
+    attention = attention or ("bf16" if precision == "bf16" else "int8")
     kpatch = cfg.get("in_dim", 16) * math.prod(cfg.get("patch_size", (1, 2, 2)))
     per_layer = 8 * C * C + 2 * C * F + 8 * C + C + F + 2 * C + 4 * C + 6 * C    # linears, biases, norms, modulation
     outside = (kpatch * C + C) + (cfg["text_dim"] * C + C * C + 2 * C) + (cfg.get("freq_dim", 256) * C + C * C + 2 * C) \
         + (6 * C * C + 6 * C) + (C * cfg.get("out_dim", 16) * math.prod(cfg.get("patch_size", (1, 2, 2))) + 2 * C + 64)
     params = 2 * (nl * per_layer + outside)
-    if precision == "fp8":
+    mx = lambda rows, cols: sum(H.mxfp4_bytes(rows, cols))
+    if precision == "mxfp4":
+        copies = nl * (2 * (2 * C * C + 2 * C) + 2 * (4 * C + F) + mx(3 * C, C) + 3 * mx(C, C) + mx(F, C) + mx(C, F))
+    elif precision == "fp8":
         copies = nl * (2 * (2 * C * C + 2 * C) + (6 * C * C + 2 * C * F) + 4 * (8 * C + 2 * F))
     else:
         copies = nl * 2 * (5 * C * C + 5 * C)
@@ -177,7 +181,10 @@ def planned_bytes(cfg, grid, seq_len, nb, text_len, sp=1, precision="bf16", atte
     M = nb * S
     n_tok = grid[0] * grid[1] * grid[2]
     ws = M * C * 4 + M * 3 * C * 2 + M * C * 2 + M * C * 2 + M * C * 4 + n_tok * kpatch * 2     # x, qkv, att, res, y, rows
-    ws += (2 * M * C + 8 * M + M * F) if precision == "fp8" else (M * C * 2 + M * F * 2)        # h / att / ffn operands
+    if precision == "mxfp4":                                                                    # h / att / ffn operands
+        ws += M * C * 2 + 2 * mx(M, C) + mx(M, F)
+    else:
+        ws += (2 * M * C + 8 * M + M * F) if precision == "fp8" else (M * C * 2 + M * F * 2)
     ws += nl * 6 * C * 4 + attn_workspace
     if attention == "int8":
         ws += 2 * nb * seq_len * (C // sp) + 4 * nb * seq_len * (N // sp) + 4 * nb * -(-seq_len // 64) * (N // sp)
@@ -194,14 +201,16 @@ class DiTEngine:
         precision: "bf16" (the reference's arithmetic) or "fp8": the six large linear layers of
         every block run on e4m3 operands - weights quantised once with a scale per output
         channel, activations per token row inside the kernel that produces them (the GELU output
-        with the fixed scale `ffn_act_scale`).
+        with the fixed scale `ffn_act_scale`); "mxfp4": the same layers on MXFP4 operands (4-bit
+        elements, one power-of-two scale per 32 values along the row; mxfp4.py), activations
+        quantised per call, the GELU output inside the product.
         attention: "bf16", or "int8": self-attention computes Q K^T on int8 operands (q with a scale per
         token and head, k per 64-key tile and head; softmax, P and P V unchanged); default: "int8"
-        with precision "fp8", else "bf16".  Cross-attention, norms, the residual stream and the head
+        with precision "fp8" or "mxfp4", else "bf16".  Cross-attention, norms, the residual stream and the head
         are the same in every mode."""
-        if precision not in ("bf16", "fp8"):
-            raise ValueError(f"precision must be 'bf16' or 'fp8', got {precision!r}")
-        attention = attention or ("int8" if precision == "fp8" else "bf16")
+        if precision not in ("bf16", "fp8", "mxfp4"):
+            raise ValueError(f"precision must be 'bf16', 'fp8' or 'mxfp4', got {precision!r}")
+        attention = attention or ("bf16" if precision == "bf16" else "int8")
         if attention not in ("bf16", "int8"):
             raise ValueError(f"attention must be 'bf16' or 'int8', got {attention!r}")
         self.precision, self.attention = precision, attention
@@ -247,6 +256,10 @@ class DiTEngine:
                 for name in FP8_LINEARS:
                     L["w8_" + name], L["s_" + name] = H.quant_rows_fp8(L["w_" + name])
                     L["w_" + name] = None            # the bf16 copy is not read again
+            elif precision == "mxfp4":
+                for name in FP8_LINEARS:
+                    L["w4_" + name] = mxfp4_quantize(L["w_" + name])
+                    L["w_" + name] = None
             self.layers.append(L)
             mods.append(L["mod"].data_ptr())
         self.mod_ptrs = torch.tensor(mods, dtype=torch.int64, device=self.device)
@@ -288,6 +301,11 @@ class DiTEngine:
             self.att8, self.att_scale = e(M, C, dt=torch.uint8), e(M, dt=F32)
             self.ffn8 = e(M, F, dt=torch.uint8)
             self.h = self.ffn = None
+        elif self.precision == "mxfp4":
+            self.h = e(M, C)
+            self.h4, self.ffn4 = MXFP4Matrix.empty(M, C, dev), MXFP4Matrix.empty(M, F, dev)
+            self.att4 = MXFP4Matrix.empty(M, C, dev)
+            self.ffn = None
         else:
             self.h = e(M, C)
             self.ffn = e(M, F)
@@ -484,6 +502,17 @@ class DiTEngine:
             H.layernorm_modulate_fp8(x2, self.h8, self.h_scale, self.eps, **kw)
         else:
             H.layernorm_modulate(x2, self.h, self.eps, **kw)
+        if self.precision == "mxfp4":
+            H.mxfp4_quant(self.h, self.h4)
+
+    def _linear_from_norm(self, L, name, out):
+        """out = Linear(normalised activations) in bf16 (the q, k, v projections, model.py:137-139, 169)."""
+        if self.precision == "fp8":
+            H.gemm_fp8(self.h8, L["w8_" + name], L["s_" + name], out, L["b_" + name], H.EPI_BF16, a_scale=self.h_scale)
+        elif self.precision == "mxfp4":
+            H.gemm_mxfp4(self.h4, L["w4_" + name], out, L["b_" + name], H.EPI_BF16)
+        else:
+            H.gemm(self.h, L["w_" + name], out, L["b_" + name], H.EPI_BF16)
 
     def _linear_from_attention(self, att2, L, name):
         """self.res = Linear(attention output) in bf16 (the o projections, model.py:152, 177)."""
@@ -491,6 +520,8 @@ class DiTEngine:
             H.quant_rows_fp8(att2, self.att8, self.att_scale)
             H.gemm_fp8(self.att8, L["w8_" + name], L["s_" + name], self.res, L["b_" + name], H.EPI_BF16,
                        a_scale=self.att_scale)
+        elif self.precision == "mxfp4":
+            H.gemm_mxfp4(H.mxfp4_quant(att2, self.att4), L["w4_" + name], self.res, L["b_" + name], H.EPI_BF16)
         else:
             H.gemm(att2, L["w_" + name], self.res, L["b_" + name], H.EPI_BF16)
 
@@ -534,10 +565,7 @@ class DiTEngine:
             mod = self.mod[l]
             # self-attention (model.py:242-246)
             self._norm(x2, pending, shift=mod[0], scale=mod[1], round_norm=(l == 0))
-            if fp8:
-                H.gemm_fp8(self.h8, L["w8_qkv"], L["s_qkv"], qkv2, L["b_qkv"], H.EPI_BF16, a_scale=self.h_scale)
-            else:
-                H.gemm(self.h, L["w_qkv"], qkv2, L["b_qkv"], H.EPI_BF16)
+            self._linear_from_norm(L, "qkv", qkv2)
             if self.sp > 1:
                 self._self_attention_sp(L)
             else:
@@ -548,10 +576,7 @@ class DiTEngine:
             # cross-attention (model.py:250): local query rows against the replicated context K/V
             self._norm(x2, pending, weight=L["n3w"], bias=L["n3b"])
             qc = qkv2[:, :C]
-            if fp8:
-                H.gemm_fp8(self.h8, L["w8_cq"], L["s_cq"], qc, L["b_cq"], H.EPI_BF16, a_scale=self.h_scale)
-            else:
-                H.gemm(self.h, L["w_cq"], qc, L["b_cq"], H.EPI_BF16)
+            self._linear_from_norm(L, "cq", qc)
             H.rmsnorm_rope(qc, L["cnq"], qc, D, self.eps)
             kvl = ctx.kv[l]
             # (the workspace only matters for long contexts - V2V with thousands of visual tokens - and
@@ -568,6 +593,9 @@ class DiTEngine:
                            out_scale=self.ffn_act_scale)
                 H.gemm_fp8(self.ffn8, L["w8_f2"], L["s_f2"], self.res, L["b_f2"], H.EPI_BF16,
                            a_scale_all=self.ffn_act_scale)
+            elif self.precision == "mxfp4":
+                H.gemm_mxfp4_gelu(self.h4, L["w4_f0"], self.ffn4, L["b_f0"])
+                H.gemm_mxfp4(self.ffn4, L["w4_f2"], self.res, L["b_f2"], H.EPI_BF16)
             else:
                 H.gemm(self.h, L["w_f0"], self.ffn, L["b_f0"], H.EPI_BF16_GELU)
                 H.gemm(self.ffn, L["w_f2"], self.res, L["b_f2"], H.EPI_BF16)

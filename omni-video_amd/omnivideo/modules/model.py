@@ -289,10 +289,10 @@ class WanModel(nn.Module):
         self._engine_key = None
         self._ctx_key = None
         self._ctx_cache = None
-        # "bf16" = the reference's arithmetic; "fp8" = e4m3 operands for the six large linear layers of
-        # every block (an extension: the reference has no such mode).  Takes effect at the next forward.
+        # "bf16" = the reference's arithmetic; "fp8" = e4m3 operands, "mxfp4" = 4-bit MXFP4 operands for the six large
+        # linear layers of every block (extensions: the reference has no such modes).  Takes effect at the next forward.
         self.linear_precision = "bf16"
-        # self-attention operands: "auto" = int8 Q K^T in the fp8 mode, bf16 otherwise; "bf16" / "int8" force one
+        # self-attention operands: "auto" = bf16, int8 Q K^T in the fp8 and mxfp4 modes; "bf16" / "int8" force one
         self.attention_precision = "auto"
 
     # ---- diffusers-layout directories -----------------------------------------------

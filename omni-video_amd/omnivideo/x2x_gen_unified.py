@@ -184,7 +184,7 @@ class OmniVideoX2XUnified:
                  visual_context_adapter_patch_size=(1, 4, 4), max_context_len=None, init_on_cpu=True,
                  wan_config=None, fsdp_shard_size=None, *, linear_precision="bf16"):
         """linear_precision (extension): "bf16" = the reference's arithmetic; "fp8" runs the six large
-        linear layers of every DiT block on e4m3 operands (WanModel.linear_precision)."""
+        linear layers of every DiT block on e4m3 operands, "mxfp4" on 4-bit MXFP4 operands (WanModel.linear_precision)."""
         self.linear_precision = linear_precision
         self.device = torch.device(f"cuda:{device_id}")
         self.config, self.rank, self.t5_cpu, self.dit_fsdp, self.init_on_cpu = config, rank, t5_cpu, dit_fsdp, init_on_cpu
