@@ -33,20 +33,21 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
     const uint32_t e = amax_bits >> 23;                   // biased exponent; 255: infinity or NaN
     return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
 }
-// 2^(127 - s) as a float (s <= 252; 255 never reaches a finite value, its codes do not matter)
-__device__ __forceinline__ float inv_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+// the scale as the conversion to codes takes it: a float of that exponent field (0: 2^-127).  255 is a NaN's; the codes of
+// such a block do not matter
+__device__ __forceinline__ float cvt_scale(uint32_t s) { return __uint_as_float(s << 23); }
 // 2^(s - 127); s = 0 is the denormal 2^-127, s = 255 a NaN
 __device__ __forceinline__ float scale_value(uint32_t s) {
     return __uint_as_float(s == 0u ? 0x00400000u : (s == 255u ? 0x7FC00000u : s << 23));
 }
 
-// eight floats (already divided by their scale) -> eight codes, k ascending from the low nibble
-__device__ __forceinline__ uint32_t pack_fp4x8(const float (&v)[8]) {
+// eight floats divided by `scale` -> eight codes, k ascending from the low nibble
+__device__ __forceinline__ uint32_t pack_fp4x8(const float* v, float scale) {
     uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], 1.0f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], 1.0f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], 1.0f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], 1.0f, 3);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
     return w;
 }
 
@@ -109,10 +110,7 @@ __global__ void __launch_bounds__(256) mxfp4_quant_kernel(const T* __restrict__ 
             mx = umax(mx, __shfl_xor(mx, 1, 64));
             mx = umax(mx, __shfl_xor(mx, 2, 64));
             const uint32_t s = scale_byte(mx);
-            const float inv = inv_scale(s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[ks][j] *= inv;
-            *reinterpret_cast<uint32_t*>(dst + ks * FRAG + r * 16) = pack_fp4x8(v[ks]);
+            *reinterpret_cast<uint32_t*>(dst + ks * FRAG + r * 16) = pack_fp4x8(v[ks], cvt_scale(s));
             sc |= s << (8 * ks);
         }
         if ((c & 3) == 0) sdst[r] = sc;
@@ -173,17 +171,21 @@ struct Out {
     const float* gate;
 };
 
-// four consecutive columns n .. n + 3 (n % 4 == 0, n < N) of row m; the pre-activation stays in fp32: the only
-// rounding is that of the stored value
+// bias of columns n .. n + 3 (n % 4 == 0; past N: some other columns', for outputs that are not stored)
+__device__ __forceinline__ uint2 load_bias(const Out& o, int n, int N) {
+    return o.bias ? *reinterpret_cast<const uint2*>(o.bias + min(n, N - 4)) : make_uint2(0, 0);
+}
+__device__ __forceinline__ void add_bias(float (&y)[4], const uint2& b) {
+    y[0] += bf2f(b.x & 0xffff);
+    y[1] += bf2f(b.x >> 16);
+    y[2] += bf2f(b.y & 0xffff);
+    y[3] += bf2f(b.y >> 16);
+}
+
+// four consecutive columns n .. n + 3 (n % 4 == 0, n < N) of row m, bias added; the pre-activation stays in fp32: the
+// only rounding is that of the stored value
 template <int EPI>
 __device__ __forceinline__ void store4(const Out& o, long m, int n, float (&y)[4]) {
-    if (o.bias) {
-        const uint2 b = *reinterpret_cast<const uint2*>(o.bias + n);
-        y[0] += bf2f(b.x & 0xffff);
-        y[1] += bf2f(b.x >> 16);
-        y[2] += bf2f(b.y & 0xffff);
-        y[3] += bf2f(b.y >> 16);
-    }
     if constexpr (EPI == EPI_BF16 || EPI == EPI_BF16_GELU) {
         if constexpr (EPI == EPI_BF16_GELU) {
 #pragma unroll
@@ -206,21 +208,18 @@ __device__ __forceinline__ void store4(const Out& o, long m, int n, float (&y)[4
 // EPI_MX_GELU: the 32 x 32 block of outputs that a wave holds in `acc` (register 4 g + j of lane l: row l & 31, column
 // 8 g + 4 (l >> 5) + j) through bias and GELU and, still in fp32, into one MX block per row of the next product's operand:
 // a row's 32 values lie in two lanes, so its largest magnitude is 15 maxima and one exchange, and each lane ends up with
-// the whole 16 bytes of codes.  o.out: the codes, o.gate: the scales (as addresses), N columns, out_groups k-groups a row
-// block.  Columns past N are written as zeros: they are the padding of that operand.
-__device__ __forceinline__ void store_mx(const Out& o, const f32x16& acc, long rb, int nb, long m, int M, int N, int out_groups,
-                                         int lane) {
+// the whole 16 bytes of codes, stored here (o.out, N columns, out_groups k-groups a row block).  Returns the block's scale
+// byte.  Columns past N are written as zeros: they are the padding of that operand.
+__device__ __forceinline__ uint32_t store_mx(const Out& o, const f32x16& acc, const uint2 (&bias)[4], long rb, int nb, long m, int M,
+                                         int N, int out_groups, int lane) {
     const int h = lane >> 5;
     float y[16];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const int n = nb * 32 + 8 * g + 4 * h;
-        uint2 b = make_uint2(0, 0);
-        if (o.bias && n < N) b = *reinterpret_cast<const uint2*>(o.bias + n);
-        y[4 * g] = acc[4 * g] + bf2f(b.x & 0xffff);
-        y[4 * g + 1] = acc[4 * g + 1] + bf2f(b.x >> 16);
-        y[4 * g + 2] = acc[4 * g + 2] + bf2f(b.y & 0xffff);
-        y[4 * g + 3] = acc[4 * g + 3] + bf2f(b.y >> 16);
+        float t[4] = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+        add_bias(t, bias[g]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * g + j] = t[j];
     }
     uint32_t mx = 0;
 #pragma unroll
@@ -230,19 +229,7 @@ __device__ __forceinline__ void store_mx(const Out& o, const f32x16& acc, long r
     }
     const auto ex = __builtin_amdgcn_permlane32_swap(mx, mx, false, false);
     const uint32_t s = scale_byte(umax(ex[0], ex[1]));
-    const float inv = inv_scale(s);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] *= inv;
-    uint32_t w[2];                       // this lane's codes: 4 g + j ascending, 16 bits per g
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        uint32_t u = 0;
-        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q], y[8 * q + 1], 1.0f, 0);
-        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 2], y[8 * q + 3], 1.0f, 1);
-        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 4], y[8 * q + 5], 1.0f, 2);
-        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, y[8 * q + 6], y[8 * q + 7], 1.0f, 3);
-        w[q] = u;
-    }
+    const uint32_t w[2] = {pack_fp4x8(y, cvt_scale(s)), pack_fp4x8(y + 8, cvt_scale(s))};      // 4 g + j ascending, 16 bits per g
     // word g of the block = columns 8 g .. 8 g + 7: 16 bits from the lower lane, 16 from the upper
     const auto e0 = __builtin_amdgcn_permlane32_swap(w[0], w[0], false, false);
     const auto e1 = __builtin_amdgcn_permlane32_swap(w[1], w[1], false, false);
@@ -251,10 +238,11 @@ __device__ __forceinline__ void store_mx(const Out& o, const f32x16& acc, long r
         *reinterpret_cast<uint4*>(data + ((nb & 1) * 32 + (lane & 31)) * 16) =
             make_uint4((e0[0] & 0xffffu) | (e0[1] << 16), (e0[0] >> 16) | (e0[1] & 0xffff0000u),
                        (e1[0] & 0xffffu) | (e1[1] << 16), (e1[0] >> 16) | (e1[1] & 0xffff0000u));
-        uint8_t* scale = reinterpret_cast<uint8_t*>(const_cast<float*>(o.gate)) + (rb * out_groups + (nb >> 3)) * GRP_SCALE;
-        scale[((nb & 1) * 32 + (lane & 31)) * 4 + ((nb >> 1) & 3)] = (uint8_t)s;
     }
+    return s;
 }
+// the scale buffer of an MXFP4 output (o.gate holds its address)
+__device__ __forceinline__ uint8_t* mx_scales(const Out& o) { return reinterpret_cast<uint8_t*>(const_cast<float*>(o.gate)); }
 
 // one 32-row x 256-k group of an operand in registers
 struct Group {
@@ -356,7 +344,14 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
             t[4 * g + 3] = y.w;
         }
         const long rb = rb0 + wave / NT;
-        store_mx(o, t, rb, (int)(nb0 + wave % NT), rb * 32 + (lane & 31), A.rows, W.rows, (W.rows + KG - 1) / KG, lane);
+        uint2 bias[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) bias[g] = load_bias(o, (int)(nb0 + wave % NT) * 32 + 8 * g + 4 * (lane >> 5), W.rows);
+        const int nb = (int)(nb0 + wave % NT), out_groups = (W.rows + KG - 1) / KG;
+        const long m = rb * 32 + (lane & 31);
+        const uint32_t sb = store_mx(o, t, bias, rb, nb, m, A.rows, W.rows, out_groups, lane);
+        if (lane < 32 && m < A.rows)
+            mx_scales(o)[(rb * out_groups + (nb >> 3)) * GRP_SCALE + ((nb & 1) * 32 + lane) * 4 + ((nb >> 1) & 3)] = (uint8_t)sb;
         return;
     }
     for (int q = wave; q < Q; q += 8) {
@@ -373,6 +368,7 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
         const long m = (rb0 + i) * 32 + (lane & 31);
         const int n = (int)(nb0 + j) * 32 + 8 * g + 4 * (lane >> 5);
         if constexpr (EPI != EPI_MX_GELU) {
+            add_bias(y, load_bias(o, n, W.rows));
             if (m < A.rows && n < W.rows) store4<EPI>(o, m, n, y);
         }
     }
@@ -411,11 +407,9 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
         mx = umax(mx, __shfl_xor(mx, 1, 64));
         mx = umax(mx, __shfl_xor(mx, 2, 64));
         const uint32_t s = scale_byte(mx);
-        const float inv = inv_scale(s);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
         const int kg = c >> 5, ks = (c >> 3) & 3, hh = (c >> 2) & 1;
-        *reinterpret_cast<uint32_t*>(codes + ((kg * 4 + ks) * 2 + hh) * (FEW_ROWS * 16) + m * 16 + (c & 3) * 4) = pack_fp4x8(v);
+        *reinterpret_cast<uint32_t*>(codes + ((kg * 4 + ks) * 2 + hh) * (FEW_ROWS * 16) + m * 16 + (c & 3) * 4) =
+            pack_fp4x8(v, cvt_scale(s));
         if ((c & 3) == 0) scales[((kg * 2 + hh) * FEW_ROWS + m) * 4 + ks] = (char)s;
     }
     __syncthreads();
@@ -447,6 +441,7 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
         y[3] += p.w;
     }
     const int n = blockIdx.x * 32 + 8 * wave + 4 * h;
+    add_bias(y, load_bias(o, n, W.rows));
     if (r < M && n < W.rows) store4<EPI>(o, r, n, y);
 }
 
@@ -599,6 +594,19 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
     }
     const int a_rd = wr * 2 * GRP_DATA, w_rd = wc * GRP_DATA;
     const int sa_rd = wr * 2 * GRP_SCALE + lane * 4, sw_rd = wc * GRP_SCALE + lane * 4;
+    uint2 bias[2][4];                    // loaded ahead of the DMA: no ordinary load waits behind it
+    if (o.bias) {
+#pragma unroll
+        for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                bias[nh][g] = *reinterpret_cast<const uint2*>(o.bias + min(col0 + nh * 128 + wc * 32 + 8 * g + 4 * (lane >> 5), W.rows - 4));
+    } else {
+#pragma unroll
+        for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) bias[nh][g] = make_uint2(0, 0);
+    }
     f32x16 acc[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -629,78 +637,84 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
     asm volatile("" ::: "memory");
 
     // acc[nh][mh * 2 + mb] register 4 g + j is out[m][n + j], m = row0 + mh * 128 + wr * 64 + mb * 32 + (lane & 31),
-    // n = col0 + nh * 128 + wc * 32 + 8 g + 4 (lane >> 5).  bf16 rows go through LDS (128 rows of 512 bytes per half,
-    // chunk c of row r at c ^ (r & 15)) so that 32 lanes store one 512-byte row segment.
+    // n = col0 + nh * 128 + wc * 32 + 8 g + 4 (lane >> 5).  bf16 rows go through LDS (256 rows of 512 bytes, chunk c of row r
+    // at c ^ (r & 15)) so that 32 lanes store one 512-byte row segment.
     constexpr bool NARROW = EPI == EPI_BF16 || EPI == EPI_BF16_GELU;
     const int fr = lane & 31, fh = lane >> 5;
     if constexpr (EPI == EPI_MX_GELU) {          // a tile's 256 columns are one k-group of the next operand
+        // (the scale bytes of a row's group come from four waves: they meet in LDS, [row block][lane][4] as in memory)
         const int out_groups = (W.rows + KG - 1) / KG;
 #pragma unroll
-        for (int mh = 0; mh < 2; ++mh)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int mb = 0; mb < 2; ++mb)
+            for (int nh = 0; nh < 2; ++nh) {
+                const int rbl = (q >> 1) * 4 + wr * 2 + (q & 1);
+                const long rb = tm * 8 + rbl;
+                const uint32_t sb = store_mx(o, acc[nh][q], bias[nh], rb, tn * 8 + nh * 4 + wc, rb * 32 + fr, A.rows, W.rows, out_groups,
+                                             lane);
+                if (fh == 0) smem[rbl * GRP_SCALE + ((wc & 1) * 32 + fr) * 4 + nh * 2 + (wc >> 1)] = (char)sb;
+            }
+        __syncthreads();
+        const long rb = tm * 8 + wave;
+        if (rb * 32 + fr < A.rows)
+            reinterpret_cast<uint32_t*>(mx_scales(o) + (rb * out_groups + tn) * GRP_SCALE)[lane] =
+                reinterpret_cast<const uint32_t*>(smem + wave * GRP_SCALE)[lane];
+    } else if (NARROW && wide) {
 #pragma unroll
-                for (int nh = 0; nh < 2; ++nh) {
-                    const long rb = tm * 8 + mh * 4 + wr * 2 + mb;
-                    store_mx(o, acc[nh][mh * 2 + mb], rb, tn * 8 + nh * 4 + wc, rb * 32 + fr, A.rows, W.rows, out_groups, lane);
-                }
-        return;
-    }
-    const bool staged = NARROW && wide;
-#pragma unroll
-    for (int mh = 0; mh < 2; ++mh) {
-        char* img = smem + mh * PBUF;
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-            const int rl = wr * 64 + mb * 32 + fr;
-            const long m = row0 + mh * 128 + rl;
-            if (!staged && m >= A.rows) continue;
+        for (int q = 0; q < 4; ++q)              // mh * 2 + mb
 #pragma unroll
             for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int nl = nh * 128 + wc * 32 + 8 * g + 4 * fh;
-                    const int n = col0 + nl;
-                    const f32x16& a16 = acc[nh][mh * 2 + mb];
+                    const f32x16& a16 = acc[nh][q];
                     float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
-                    if (!staged) {
-                        if constexpr (EPI != EPI_MX_GELU) {
-                            if (n < W.rows) store4<EPI>(o, m, n, y);
-                        }
-                        continue;
-                    }
-                    if (o.bias) {
-                        const uint2 b = *reinterpret_cast<const uint2*>(o.bias + min(n, W.rows - 4));
-                        y[0] += bf2f(b.x & 0xffff);
-                        y[1] += bf2f(b.x >> 16);
-                        y[2] += bf2f(b.y & 0xffff);
-                        y[3] += bf2f(b.y >> 16);
-                    }
+                    add_bias(y, bias[nh][g]);
                     if constexpr (EPI == EPI_BF16_GELU) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = gelu_tanh_f(y[j]);
                     }
-                    *reinterpret_cast<uint2*>(img + rl * 512 + (((nl >> 3) ^ (rl & 15)) << 4) + fh * 8) =
+                    const int rl = (q >> 1) * 128 + wr * 64 + (q & 1) * 32 + fr, c = nh * 16 + wc * 4 + g;
+                    *reinterpret_cast<uint2*>(smem + rl * 512 + ((c ^ (rl & 15)) << 4) + fh * 8) =
                         make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
                 }
-        }
-        if (staged) {       // uniform: every thread reaches the barrier
-            __syncthreads();
-            const int rr = tid >> 5, cc = tid & 31;
-            const int n = col0 + cc * 8;
-            bf16_t* ob = reinterpret_cast<bf16_t*>(o.out) + n;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 16 + rr;
-                const long m = row0 + mh * 128 + r;
-                const uint4 v = *reinterpret_cast<const uint4*>(img + r * 512 + ((cc ^ (r & 15)) << 4));
-                if (m < A.rows) {
+        __syncthreads();
+        const int rr = tid >> 5, cc = tid & 31;
+        const int n = col0 + cc * 8;
+        const char* img = smem + rr * 512 + ((cc ^ rr) << 4);                 // row r = 16 i + rr: r & 15 = rr
+        bf16_t* ob = reinterpret_cast<bf16_t*>(o.out) + (row0 + rr) * o.ldo + n;
+        const long step = 16 * o.ldo;
+        if (row0 + TM <= A.rows && col0 + TN <= W.rows) {                     // uniform
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(img + i * 8192);
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(ob));
+                ob += step;
+            }
+        } else {
+            for (int i = 0; i < 16; ++i, ob += step) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(img + i * 8192);
+                if (row0 + i * 16 + rr < A.rows) {
                     if (n + 8 <= W.rows)
-                        __builtin_nontemporal_store((u32x4){v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(ob + m * o.ldo));
+                        __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(ob));
                     else if (n < W.rows)
-                        *reinterpret_cast<uint2*>(ob + m * o.ldo) = make_uint2(v.x, v.y);
+                        *reinterpret_cast<uint2*>(ob) = make_uint2(v[0], v[1]);
                 }
             }
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const long m = row0 + (q >> 1) * 128 + wr * 64 + (q & 1) * 32 + fr;
+#pragma unroll
+            for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int n = col0 + nh * 128 + wc * 32 + 8 * g + 4 * fh;
+                    const f32x16& a16 = acc[nh][q];
+                    float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
+                    add_bias(y, bias[nh][g]);
+                    if (m < A.rows && n < W.rows) store4<EPI>(o, m, n, y);
+                }
         }
     }
 }

@@ -797,7 +797,7 @@ def gemm_mxfp4_gelu(a, w, out, bias=None):
     return out
 
 
-MXFP4_FEW_ROWS = 8           # up to this many rows linear_mxfp4 quantises inside the product (one launch)
+MXFP4_FEW_ROWS, MXFP4_FEW_K = 8, 16384      # up to this many rows and columns linear_mxfp4 needs no workspace (one launch)
 
 
 def linear_mxfp4(x, w, out, bias=None, epilogue=EPI_BF16, gate=None):
@@ -811,8 +811,8 @@ def linear_mxfp4(x, w, out, bias=None, epilogue=EPI_BF16, gate=None):
     if not M:
         return out
     ws, ws_ptr, nb = None, None, 0
-    if M > MXFP4_FEW_ROWS or K > 16384:
-        nb = int(lib().ovd_linear_mxfp4_workspace_bytes(M, K))
+    if M > MXFP4_FEW_ROWS or K > MXFP4_FEW_K:
+        nb = sum(mxfp4_bytes(M, K))
         ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
         ws_ptr = ws.data_ptr()
     wd, wsc = w.pointers()
