@@ -5,7 +5,7 @@ import re
 
 import pytest
 
-from test_isa_schedule import CSRC, HIPCC, kernels
+from test_isa_schedule import CSRC, HIPCC
 
 FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -17,6 +17,12 @@ def listing(src, tmp_path, *extra):
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fno-gpu-rdc", "-S", "--cuda-device-only", *FLAGS,
                     *extra, os.path.join(CSRC, src), "-o", str(out)], check=True, capture_output=True)
     return out.read_text()
+
+
+def kernels(text, name):
+    """{mangled name: whole body} of the instantiations of `name`"""
+    return {m.group(1): text[m.end():text.index(".end_amdhsa_kernel", m.end())]
+            for m in re.finditer(r"^(_ZN\S*%s\S*):\s" % name, text, re.M)}
 
 
 def blocks(body):
