@@ -82,7 +82,7 @@ __device__ __forceinline__ int parts_of(const Args& a, int lk) {
 
 // document, row block (of ROWS rows) and part of its keys of work item `blk`; false past the last one.  Up to SORTED
 // documents are walked from the longest keys to the shortest, so that the last workgroups to start are short ones (packed
-// prompts of 1 to 2100 tokens, 4 key heads: 92 us in the order given, 66 sorted); more are taken in their order.
+// prompts of 1 to 2100 tokens, 4 key heads: 92 us in the order given, 77 sorted); more are taken in their order.
 constexpr int SORTED = 32;
 
 template <int ROWS, bool SPLIT>
@@ -719,16 +719,29 @@ struct Plan {
     int row_blocks, chunk, max_splits;
 };
 
-Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, int D, long max_q, long max_k) {
+// 8 waves (256 rows, one workgroup per CU) or 4 (128 rows, two that overlap each other's start and end)?  Eight read K and
+// V half as often and are 7 % faster in full rounds, but a last round that is partly filled costs them a whole one.
+//   short keys: four (60 documents of 257 tokens, 12 heads: 80 us against 98);
+//   causal (lengths differ, longest first): four below three rounds of eight (packed prompts of 1 to 2100 tokens with a cap
+//   68 us against 77; 6000 tokens, 12 heads 134 against 143; 20280 tokens, 12 heads: 1239 against 1188);
+//   otherwise by rounds, a round of four-wave workgroups that run alone on their CUs counted as 0.6 (6000 tokens, 12
+//   heads: 274 us against 297; three documents of 3000: 183 against 166; 20280: 2331 against 2151).
+bool wide_workgroups(long rows, int docs, int kv_heads, int causal, long max_k, long cus) {
+    const long w8 = (rows / 256 + (docs + 1) / 2) * kv_heads, w4 = (rows / 128 + (docs + 1) / 2) * kv_heads;
+    if (max_k <= 1024) return false;
+    if (causal) return w8 >= 3 * cus;
+    const double rem = (double)(w4 % (2 * cus)) / cus;
+    const double t4 = 1.07 * ((double)(w4 / (2 * cus)) + (rem == 0 ? 0. : rem <= 1. ? 0.6 : 1.));
+    return (double)((w8 + cus - 1) / cus) < t4;
+}
+
+Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, int D, long max_q, long max_k, int causal) {
     Plan p;
     const long cus = ovd_device_cus();
     max_q = max_q < 1 ? 1 : (max_q > total_q ? total_q : max_q);
     max_k = max_k < 1 ? 1 : (max_k > total_k ? (total_k < 1 ? 1 : total_k) : max_k);
     const long rows = max_q * group;
-    // 256-row workgroups when they fill the chip and the documents are long, 128 rows otherwise (two workgroups of a CU
-    // then overlap each other's start and end: 60 documents of 257 tokens 76 us against 101, queries of 34320 tokens
-    // over 131 and 550 keys 118 against 125), one wave when 32 rows hold a document's queries
-    p.waves = rows <= 32 ? 1 : (max_k > 1024 && total_q * group / 256 * kv_heads >= cus ? 8 : 4);
+    p.waves = rows <= 32 ? 1 : (wide_workgroups(total_q * group, docs, kv_heads, causal, max_k, cus) ? 8 : 4);
     const long per = 32L * p.waves;
     p.row_blocks = (int)(total_q * group / per + docs);        // >= the sum of ceil(Lq group / per) over the documents
     p.split = p.waves == 1 || (p.waves == 4 && (long)p.row_blocks * kv_heads <= cus);
@@ -768,8 +781,12 @@ Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, int 
 long ovd_impl_attn_packed_workspace(long total_q, long total_k, int docs, int q_heads, int kv_heads, int D, long max_q,
                                     long max_k) {
     if (total_q <= 0 || docs <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads) return 0;
-    const Plan p = plan_of(total_q, total_k, docs, kv_heads, q_heads / kv_heads, D, max_q, max_k);
-    return p.max_splits > 1 ? (long)p.max_splits * total_q * q_heads * (D + 2) * (long)sizeof(float) : 0;
+    int parts = 1;
+    for (int causal = 0; causal < 2; ++causal) {
+        const Plan p = plan_of(total_q, total_k, docs, kv_heads, q_heads / kv_heads, D, max_q, max_k, causal);
+        if (p.max_splits > parts) parts = p.max_splits;
+    }
+    return parts > 1 ? (long)parts * total_q * q_heads * (D + 2) * (long)sizeof(float) : 0;
 }
 
 int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* out, long total_q, long total_k,
@@ -803,7 +820,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.cap_in = softcap > 0.f ? 2.f * a.scale_log2 / softcap : 0.f;
     a.cap_out = softcap * 1.4426950408889634f;
-    const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, D, max_q, max_k);
+    const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, D, max_q, max_k, causal);
     // no (or too small a) workspace: every document in one part
     const long part_bytes = total_q * q_heads * (D + 2) * (long)sizeof(float);
     const long room = workspace == nullptr ? 0 : workspace_bytes / part_bytes;
