@@ -323,7 +323,8 @@ int ovd_flash_attn_qk8_fwd_bf16(const int8_t* q8, const float* q_scale, const in
  *   stored value.  N % 4 == 0, K % 32 == 0, ldo % 4 == 0; bias bf16 [N] or NULL.  Sums are in a fixed order.
  * ovd_linear_mxfp4: ovd_mxfp4_quant of x [M, K] and ovd_gemm_mxfp4 in one call, a single launch for up to 8 rows;
  *   workspace: ovd_linear_mxfp4_workspace_bytes(M, K) (HOST) bytes, 16-byte aligned (0: none, may be NULL), free again
- *   when the call's work has finished. */
+ *   when the call's work has finished.  out may share memory with x (x += f(x)); with few rows the call then needs
+ *   ovd_mxfp4_data_bytes + ovd_mxfp4_scale_bytes (M, K) bytes of workspace. */
 int64_t ovd_mxfp4_data_bytes(int64_t rows, int64_t K);
 int64_t ovd_mxfp4_scale_bytes(int64_t rows, int64_t K);
 int ovd_mxfp4_quant(const void* x, int x_is_f32, int64_t ldx, uint8_t* data, uint8_t* scale, int M, int K, void* stream);
@@ -355,7 +356,8 @@ int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos
  * [docs + 1], ascending; values are clamped to the tensors).  Query i of a document with Lq queries and Lk keys sees
  * its first Lk keys, with `causal` its first max(i + Lk - Lq + 1, prefix[d]) (prefix: device int32 [docs] or NULL).
  * softcap > 0: scores s become softcap * tanh(s / softcap).  A query that sees no key gets zeros; rows outside every
- * document are not written; keys and values outside a document do not enter it, whatever they hold.
+ * document are not written; keys and values outside a document do not enter it, whatever they hold.  out may be q
+ * itself (same strides).
  * max_q / max_k: the longest document as the host knows it; they choose the launch (any value gives right results).
  * workspace: with few query rows the keys are split over workgroups and joined, in
  * ovd_attn_packed_workspace_bytes(...) (HOST) bytes, 16-byte aligned; NULL or smaller: not split.  It holds no state

@@ -94,7 +94,7 @@ __device__ __forceinline__ bool find_block(const Args& a, int blk, int lane, int
             int q0, lq, k0, lk;
             doc_range(a, d, q0, lq, k0, lk);
             keys = lk;
-            n = (int)(((long)lq * a.group + ROWS - 1) / ROWS);
+            n = (int)(((unsigned)(lq * a.group) + ROWS - 1) / ROWS);
             if (SPLIT) {
                 np = parts_of(a, lk);
                 n *= np;
@@ -447,17 +447,18 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
     int q0, lq, k0, lk;
     doc_range(a, doc, q0, lq, k0, lk);
     const int prefix = a.prefix ? min(max(a.prefix[doc], 0), lk) : 0;
-    const long rows = (long)lq * a.group;
-    const long r_first = (long)rb * (32 * NW) + wave * 32;
-    const long row = min(r_first + l31, rows - 1);       // rows past the last repeat it and are not stored
-    const int tok = (int)(row / a.group), head = kvh * a.group + (int)(row % a.group);
+    const unsigned group = (unsigned)a.group;
+    const int rows = lq * a.group;                       // below 2^31 (checked on the host)
+    const int r_first = rb * (32 * NW) + wave * 32;
+    const unsigned row = (unsigned)min(r_first + l31, rows - 1);       // rows past the last repeat it and are not stored
+    const int tok = (int)(row / group), head = kvh * a.group + (int)(row % group);
     const int nvis = visible(a, tok, lq, lk, prefix);
     // visible counts grow with the row: the tile range follows from the workgroup's last row; a wave's own last row says
     // where its work ends, its first row which tiles need no mask
-    const long last_row = min((long)(rb + 1) * (32 * NW), rows) - 1;
-    const int kend = __builtin_amdgcn_readfirstlane(visible(a, (int)(last_row / a.group), lq, lk, prefix));
-    const int wend = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first + 31, rows - 1) / a.group), lq, lk, prefix));
-    const int full = __builtin_amdgcn_readfirstlane(visible(a, (int)(min(r_first, rows - 1) / a.group), lq, lk, prefix));
+    const unsigned last_row = (unsigned)min(rb * (32 * NW) + 32 * NW - 1, rows - 1);
+    const int kend = __builtin_amdgcn_readfirstlane(visible(a, (int)(last_row / group), lq, lk, prefix));
+    const int wend = __builtin_amdgcn_readfirstlane(visible(a, (int)((unsigned)min(r_first + 31, rows - 1) / group), lq, lk, prefix));
+    const int full = __builtin_amdgcn_readfirstlane(visible(a, (int)((unsigned)min(r_first, rows - 1) / group), lq, lk, prefix));
     const int nt = (kend + BKV - 1) / BKV;
     const int t0 = (int)((long)nt * part / parts), t1 = (int)((long)nt * (part + 1) / parts);
     const int tw = min(max((wend + BKV - 1) / BKV, t0), t1);     // this wave's tiles: [t0, tw)
@@ -555,7 +556,7 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
         }
     }
     // rows of the workgroup see different key counts: only then can a hidden value have been multiplied
-    const int wfull = __builtin_amdgcn_readfirstlane(visible(a, (int)((long)rb * (32 * NW) / a.group), lq, lk, prefix));
+    const int wfull = __builtin_amdgcn_readfirstlane(visible(a, (int)((unsigned)(rb * (32 * NW)) / group), lq, lk, prefix));
     if (t1 > wfull / BKV && t0 < t1) {
         int* flags = reinterpret_cast<int*>(smem);        // the tiles are free (last step's barrier)
         if (lane == 0) flags[wave] = redo;
@@ -607,9 +608,9 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
     for (int i = 0; i < 32 / RPI; ++i) {
         const int r = i * RPI + lane / CPR, c = lane % CPR;
         const uint4 w = *reinterpret_cast<const uint4*>(ep + r * ROWB + ((c ^ (r & (CPR - 1))) << 4));
-        const long rr = r_first + r;
-        if (rr < rows)
-            *reinterpret_cast<uint4*>(a.o + (q0 + rr / a.group) * a.o_ld + ((long)kvh * a.group + rr % a.group) * D + c * 8) = w;
+        const unsigned rr = (unsigned)(r_first + r);
+        if (rr < (unsigned)rows)
+            *reinterpret_cast<uint4*>(a.o + (long)(q0 + rr / group) * a.o_ld + (long)(kvh * group + rr % group) * D + c * 8) = w;
     }
 }
 
@@ -798,7 +799,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
                 "attn_packed: bad sizes Tq=%ld Tk=%ld documents=%d", total_q, total_k, docs);
     OVD_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0, "attn_packed: %d query heads over %d key heads",
                 q_heads, kv_heads);
-    OVD_REQUIRE(total_q * (q_heads / kv_heads) / 32 + docs < (1L << 31) - 256, "attn_packed: too many query rows");
+    OVD_REQUIRE(total_q * (q_heads / kv_heads) + 64L * docs < (1L << 31) - 1024, "attn_packed: too many query rows");
     OVD_REQUIRE(q_ld % 8 == 0 && k_ld % 8 == 0 && v_ld % 8 == 0 && o_ld % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(out) % 16 == 0,

@@ -64,7 +64,8 @@ def grid_positions(grids, device="cuda"):
 
 def packed_rope(x, positions, plan, out=None, inverse=False):
     """x [T, N, D] bf16 or fp32 (dense heads; the tokens may be strided), positions [T, axes] int32 or fp32 (or [T] for
-    one axis), plan a RopePlan of head_dim D.  Returns the rotated heads, in `out` if given (which may be x itself).
+    one axis), plan a RopePlan of head_dim D.  Returns the rotated heads, in `out` if given (x itself, or memory that does
+    not overlap it).
     inverse: the opposite rotation.  Positions may be of any size; results are rounded once, to x's type."""
     _no_grad(x)
     if positions.dim() == 1:
@@ -89,7 +90,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=Fa
     first max(i + Lk - Lq + 1, prefix[d]) of them (prefix int32 [documents] or None).  softcap > 0 caps the scores:
     softcap * tanh(s / softcap).  softmax_scale defaults to D ** -0.5.
     A query that sees no key gets zeros.  Rows outside every document are not written (uninitialised when `out` is not
-    given).  A key that is hidden from a query does not enter its result, whatever it and its value hold.
+    given).  A key that is hidden from a query does not enter its result, whatever it and its value hold.  `out` may be q
+    itself, but not share memory with k or v.
     max_q, max_k: the longest document as the caller knows it (default: the totals); they size the launch, any value
     gives right results.  workspace: a byte buffer of H.attn_packed_workspace_bytes(...) (default: allocated here)."""
     _no_grad(q, k, v)

@@ -297,6 +297,19 @@ def test_attention_strided_views_of_a_fused_projection(P):
     assert torch.equal(o, want) and (out[:, :N * D] == 0).all()
 
 
+def test_attention_in_place_and_without_keys(P):
+    for Lq, Lk, N, Nk in (([300, 70], [200, 9], 4, 2), ([1, 2, 1], [900, 0, 70], 8, 2)):
+        q, k, v = inputs(Lq, Lk, N, Nk, 128, 12)
+        want = P.packed_attention(q, k, v, cu(Lq), cu(Lk), max(Lq), max(Lk))
+        own = q.clone()
+        assert P.packed_attention(own, k, v, cu(Lq), cu(Lk), max(Lq), max(Lk), out=own) is own
+        assert torch.equal(own, want)
+        for causal in (False, True):
+            o = P.packed_attention(q, k[:0], v[:0], cu(Lq), torch.zeros(len(Lq) + 1, dtype=torch.int32, device="cuda"), causal=causal)
+            assert (o == 0).all()
+    assert P.packed_attention(q[:0], k, v, cu([0, 0, 0]), cu(Lk)).shape == (0, 8, 128)
+
+
 def test_attention_equals_flash_attn_on_one_document(P):
     import omnivideo._hip as H
     q, k, v = inputs([600], [600], 2, 2, 128, 5)
