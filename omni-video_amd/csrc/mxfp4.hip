@@ -284,7 +284,7 @@ template <int MT, int NT, int EPI>
 __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Operand W, Out o, int groups) {
     extern __shared__ float4 part[];          // [8 waves][MT * NT * 4 register quads][64 lanes]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long rb0 = (long)blockIdx.y * MT, nb0 = (long)blockIdx.x * NT;
+    const long rb0 = (long)blockIdx.x * MT, nb0 = (long)blockIdx.y * NT;
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -779,6 +779,13 @@ int ovd_impl_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out,
     return 0;
 }
 
+// whether the M rows of x and of the output share memory (x += f(x) on a residual stream): a product that reads x while it
+// writes its output must not run then
+static bool rows_overlap(const void* x, long x_row_bytes, long x_last, const void* out, long out_row_bytes, long out_last, int M) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(out);
+    return a < b + (M - 1) * out_row_bytes + out_last && b < a + (M - 1) * x_row_bytes + x_last;
+}
+
 static bool few_rows(int M, int K) { return M <= FEW_ROWS && mx_groups(K) * FEW_GRP + FEW_PART + 16 <= 160 * 1024; }
 
 // bytes for the quantised x of ovd_impl_linear_mxfp4 (0: it needs none)
@@ -816,11 +823,12 @@ int ovd_impl_linear_mxfp4(const void* x, int x_is_f32, long ldx, const uint8_t* 
     if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
     if (M == 0) return 0;
     OVD_REQUIRE(epilogue != EPI_MX_GELU || !few_rows(M, K), "linear_mxfp4: an MXFP4 output takes a quantised x (ovd_gemm_mxfp4)");
-    if (!few_rows(M, K)) {
-        const long nd = ovd_impl_mxfp4_data_bytes(M, K);
-        OVD_REQUIRE(workspace != nullptr && workspace_bytes >= ovd_impl_linear_mxfp4_workspace(M, K),
-                    "linear_mxfp4: %d rows of %d need %ld bytes of workspace, got %ld", M, K,
-                    ovd_impl_linear_mxfp4_workspace(M, K), workspace_bytes);
+    const int xb = x_is_f32 ? 4 : 2, ob = epilogue <= EPI_BF16_GELU ? 2 : 4;
+    if (!few_rows(M, K) || rows_overlap(x, ldx * xb, (long)K * xb, out, ldo * ob, (long)N * ob, M)) {
+        const long nd = ovd_impl_mxfp4_data_bytes(M, K), need = nd + ovd_impl_mxfp4_scale_bytes(M, K);
+        OVD_REQUIRE(workspace != nullptr && workspace_bytes >= need,
+                    "linear_mxfp4: %d rows of %d (or an output that shares memory with x) need %ld bytes of workspace, got %ld", M, K,
+                    need, workspace_bytes);
         uint8_t* data = (uint8_t*)workspace;
         if (ovd_impl_mxfp4_quant(x, x_is_f32, ldx, data, data + nd, M, K, st)) return 1;
         return ovd_impl_gemm_mxfp4(data, data + nd, w_data, w_scale, bias, out, ldo, gate, M, N, K, epilogue, st);
@@ -863,10 +871,9 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
         static OvdLdsLimit lim;                                                                                \
         if (!lim.ensure(reinterpret_cast<const void*>(&gemm_mxfp4_direct_kernel<MT, NT, E>), lds))             \
             OVD_FAIL("gemm_mxfp4: cannot reserve %zu bytes of LDS", lds);                                      \
-        const int ty = ceil_div(M, 32 * MT);                                                                   \
+        const int ty = ceil_div(E == EPI_MX_GELU ? ceil_div(N, KG) * KG : N, 32 * NT);                         \
         OVD_REQUIRE(ty <= 65535, "gemm_mxfp4: grid too large");                                                \
-        const int cols = E == EPI_MX_GELU ? ceil_div(N, KG) * KG : N;                                          \
-        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(cols, 32 * NT), ty), dim3(512), \
+        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(M, 32 * MT), ty), dim3(512),   \
                            lds, st, A, W, o, groups);                                                          \
     }
 #define BIG(E)                                                                                                 \

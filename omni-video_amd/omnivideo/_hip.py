@@ -791,6 +791,8 @@ def gemm_mxfp4_gelu(a, w, out, bias=None):
         raise ValueError(f"gemm_mxfp4: bias must be a contiguous bf16 row of length {N}")
     dev = _one_device(a.buf, w.buf, out.buf, bias)
     (ad, asc), (wd, wsc), (od, osc) = a.pointers(), w.pointers(), out.pointers()
+    if M and od in (ad, wd):
+        raise ValueError("gemm_mxfp4: the output matrix cannot be one of the operands")
     if M:
         _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), od, N, osc, M, N, K,
                  EPI_MXFP4_GELU)
@@ -811,7 +813,7 @@ def linear_mxfp4(x, w, out, bias=None, epilogue=EPI_BF16, gate=None):
     if not M:
         return out
     ws, ws_ptr, nb = None, None, 0
-    if M > MXFP4_FEW_ROWS or K > MXFP4_FEW_K:
+    if M > MXFP4_FEW_ROWS or K > MXFP4_FEW_K or x.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
         nb = sum(mxfp4_bytes(M, K))
         ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
         ws_ptr = ws.data_ptr()

@@ -128,7 +128,8 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
     """act(x @ weight.T + bias) with both operands in MXFP4 and fp32 accumulation; one rounding, of the stored value.
     x: [..., K] bf16 or fp32 (quantised here), or an MXFP4Matrix; weight: MXFP4Matrix [N, K], N a multiple of 4;
     bias bf16 [N]; gelu: tanh-GELU (bf16 output).  Returns [..., N] in out_dtype (bf16 or fp32), written to `out` if given.
-    residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned.
+    residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned; out and
+    residual may be x itself.
     quantize_output (with gelu, N a multiple of 32): the result as an MXFP4Matrix [M, N] (`out` if given), quantised from
     fp32 in the product's own pass: the input of the next layer."""
     if not isinstance(weight, MXFP4Matrix):

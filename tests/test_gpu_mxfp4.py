@@ -252,6 +252,33 @@ def test_linear_of_few_rows_equals_quantise_then_product(X, M, K, N):
     assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all()
 
 
+@pytest.mark.parametrize("M", [1, 8, 40, 700])
+def test_linear_into_its_own_input(X, M):
+    """x = f(x) and x += f(x): what is read is x as it was"""
+    C = 1536
+    w = X.mxfp4_quantize(randn((C, C), 1, 1 / math.sqrt(C)).cuda())
+    for dt in (BF16, F32):
+        x = randn((M, C), 2).to(dt).cuda()
+        want = X.mxfp4_linear(x, w, out_dtype=dt)
+        for _ in range(3):
+            y = x.clone()
+            assert X.mxfp4_linear(y, w, out=y) is y
+            assert torch.equal(y, want)
+    x = randn((M, C), 3).cuda()
+    want = X.mxfp4_linear(x, w, residual=x.clone())
+    buf = torch.zeros(M + 1, C, device="cuda")
+    for rows in (buf[:M], buf[1:]):
+        rows.copy_(x)
+        X.mxfp4_linear(rows, w, residual=rows)
+        assert torch.equal(rows, want)
+
+
+def test_quantised_output_refuses_an_operand(X):
+    a, w = X.mxfp4_quantize(randn((40, 64), 1).cuda()), X.mxfp4_quantize(randn((64, 64), 2).cuda())
+    with pytest.raises(ValueError, match="operands"):
+        X.mxfp4_linear(a, w, gelu=True, quantize_output=True, out=a)
+
+
 @pytest.mark.parametrize("M,N,K", [(5, 64, 512), (300, 1536, 256), (1500, 1280, 512), (4100, 2052, 512)])
 def test_linear_writes_only_its_rows(X, M, N, K):
     a, w, _, _ = operands(X, M, N, K, 9)

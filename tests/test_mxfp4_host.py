@@ -123,7 +123,8 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_gemm_mxfp4", p, p, p + 8, p, None, p, 8, None, 1, 8, 32, 0, None, why=b"16-byte")
     refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, None, 0, 9, 8, 32, 0, None, why=b"workspace")
     refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, p, 4351, 9, 8, 32, 0, None, why=b"workspace")
-    refused("ovd_linear_mxfp4", p, 0, 33, p, p, None, p, 8, None, None, 0, 2, 8, 32, 0, None, why=b"alignment")
+    refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p + 64, 8, None, None, 0, 2, 8, 32, 0, None, why=b"shares memory")
+    refused("ovd_linear_mxfp4", p, 0, 33, p, p, None, p + 1024, 8, None, None, 0, 2, 8, 32, 0, None, why=b"alignment")
     refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 8, None, None, 0, 2, 8, 32, 5, None, why=b"epilogue")
     assert L.ovd_linear_mxfp4_workspace_bytes(H.MXFP4_FEW_ROWS, H.MXFP4_FEW_K) == 0
     assert L.ovd_linear_mxfp4_workspace_bytes(550, 8960) == sum(H.mxfp4_bytes(550, 8960))
