@@ -54,9 +54,9 @@ __device__ __forceinline__ uint32_t pack_fp4x8(const float* v, float scale) {
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
 // ------------------------------------------------------------------------------------------ quantise / dequantise
-// One wave = one row block x one k-group.  A load instruction covers 8 rows x 64 k (8 lanes of 8 values per row: whole
-// 128-byte lines of bf16), a store instruction two runs of 8 rows x 16 bytes; the four lanes of an MX block exchange
-// their largest magnitude.  HBM-bound: 2 (4) bytes read and 17/32 written per value.
+// One workgroup = one row block x one k-group, a wave 8 of its rows.  A load instruction covers 8 rows x 64 k (8 lanes of
+// 8 values per row: whole 128-byte lines of bf16), a store instruction two runs of 8 rows x 16 bytes; the four lanes of an
+// MX block exchange their largest magnitude.  HBM-bound: 2 (4) bytes read and 17/32 written per value.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
 template <>
@@ -78,81 +78,73 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) mxfp4_quant_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ data,
-                                                          uint8_t* __restrict__ scale, int M, int K, int groups, long waves) {
+                                                          uint8_t* __restrict__ scale, int M, int K, int groups) {
     const int lane = threadIdx.x & 63;
-    const long wid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (wid >= waves) return;
+    const long wid = blockIdx.x;
     const long rb = wid / groups;
     const int kg = (int)(wid % groups);
     const int r8 = lane >> 3, c = lane & 7;               // row inside the 8-row group, 8-value chunk of the 64-k step
     uint8_t* dst = data + wid * GRP_DATA + (c >> 2) * 512 + (c & 3) * 4;
     uint32_t* sdst = reinterpret_cast<uint32_t*>(scale + wid * GRP_SCALE) + (c >> 2) * 32;
+    const int r = (threadIdx.x >> 6) * 8 + r8;
+    const long row = rb * 32 + r;
+    if (row >= M) return;                                 // eight lanes of a row share it: the exchanges stay whole
+    const T* src = x + row * ldx + (long)kg * KG + c * 8;
+    float v[4][8];
+    uint32_t sc = 0;
 #pragma unroll
-    for (int rg = 0; rg < 4; ++rg) {
-        const int r = rg * 8 + r8;
-        const long row = rb * 32 + r;
-        if (row >= M) break;
-        const T* src = x + row * ldx + (long)kg * KG + c * 8;
-        float v[4][8];
-        uint32_t sc = 0;
+    for (int ks = 0; ks < 4; ++ks) {
+        if (kg * KG + ks * 64 + c * 8 < K) load8<T>(src + ks * 64, v[ks]);
+        else
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            if (kg * KG + ks * 64 + c * 8 < K) load8<T>(src + ks * 64, v[ks]);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[ks][j] = 0.f;
-        }
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            uint32_t mx = 0;                              // magnitudes compare as their bit patterns (NaN above all)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mx = umax(mx, __float_as_uint(v[ks][j]) & 0x7fffffffu);
-            mx = umax(mx, __shfl_xor(mx, 1, 64));
-            mx = umax(mx, __shfl_xor(mx, 2, 64));
-            const uint32_t s = scale_byte(mx);
-            *reinterpret_cast<uint32_t*>(dst + ks * FRAG + r * 16) = pack_fp4x8(v[ks], cvt_scale(s));
-            sc |= s << (8 * ks);
-        }
-        if ((c & 3) == 0) sdst[r] = sc;
+            for (int j = 0; j < 8; ++j) v[ks][j] = 0.f;
     }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        uint32_t mx = 0;                              // magnitudes compare as their bit patterns (NaN above all)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = umax(mx, __float_as_uint(v[ks][j]) & 0x7fffffffu);
+        mx = umax(mx, __shfl_xor(mx, 1, 64));
+        mx = umax(mx, __shfl_xor(mx, 2, 64));
+        const uint32_t s = scale_byte(mx);
+        *reinterpret_cast<uint32_t*>(dst + ks * FRAG + r * 16) = pack_fp4x8(v[ks], cvt_scale(s));
+        sc |= s << (8 * ks);
+    }
+    if ((c & 3) == 0) sdst[r] = sc;
 }
 
 // the mapping above, the other way; a value is code * 2^(s - 127), exact in bf16 and fp32
 template <typename T>
 __global__ void __launch_bounds__(256) mxfp4_dequant_kernel(const uint8_t* __restrict__ data,
                                                             const uint8_t* __restrict__ scale, T* __restrict__ out,
-                                                            long ldo, int M, int K, int groups, long waves) {
+                                                            long ldo, int M, int K, int groups) {
     const int lane = threadIdx.x & 63;
-    const long wid = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (wid >= waves) return;
+    const long wid = blockIdx.x;
     const long rb = wid / groups;
     const int kg = (int)(wid % groups);
     const int r8 = lane >> 3, c = lane & 7;
     const uint8_t* src = data + wid * GRP_DATA + (c >> 2) * 512 + (c & 3) * 4;
     const uint32_t* ssrc = reinterpret_cast<const uint32_t*>(scale + wid * GRP_SCALE) + (c >> 2) * 32;
+    const int r = (threadIdx.x >> 6) * 8 + r8;
+    const long row = rb * 32 + r;
+    if (row >= M) return;
+    const uint32_t sc = ssrc[r];
+    T* dst = out + row * ldo + (long)kg * KG + c * 8;
 #pragma unroll
-    for (int rg = 0; rg < 4; ++rg) {
-        const int r = rg * 8 + r8;
-        const long row = rb * 32 + r;
-        if (row >= M) break;
-        const uint32_t sc = ssrc[r];
-        T* dst = out + row * ldo + (long)kg * KG + c * 8;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(src + ks * FRAG + r * 16);
-            const float s = scale_value((sc >> (8 * ks)) & 255u);
-            const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0) * s;
-            const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1) * s;
-            const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2) * s;
-            const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3) * s;
-            if (kg * KG + ks * 64 + c * 8 >= K) continue;
-            if constexpr (sizeof(T) == 2) {
-                *reinterpret_cast<uint4*>(dst + ks * 64) =
-                    make_uint4(pack_bf2(p0[0], p0[1]), pack_bf2(p1[0], p1[1]), pack_bf2(p2[0], p2[1]), pack_bf2(p3[0], p3[1]));
-            } else {
-                reinterpret_cast<float4*>(dst + ks * 64)[0] = make_float4(p0[0], p0[1], p1[0], p1[1]);
-                reinterpret_cast<float4*>(dst + ks * 64)[1] = make_float4(p2[0], p2[1], p3[0], p3[1]);
-            }
+    for (int ks = 0; ks < 4; ++ks) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(src + ks * FRAG + r * 16);
+        const float s = scale_value((sc >> (8 * ks)) & 255u);
+        const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0) * s;
+        const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1) * s;
+        const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2) * s;
+        const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3) * s;
+        if (kg * KG + ks * 64 + c * 8 >= K) continue;
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4*>(dst + ks * 64) =
+                make_uint4(pack_bf2(p0[0], p0[1]), pack_bf2(p1[0], p1[1]), pack_bf2(p2[0], p2[1]), pack_bf2(p3[0], p3[1]));
+        } else {
+            reinterpret_cast<float4*>(dst + ks * 64)[0] = make_float4(p0[0], p0[1], p1[0], p1[1]);
+            reinterpret_cast<float4*>(dst + ks * 64)[1] = make_float4(p2[0], p2[1], p3[0], p3[1]);
         }
     }
 }
@@ -277,14 +269,17 @@ __device__ __forceinline__ void mfma_group(f32x16& acc, const Group& w, const Gr
     acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.f[3]), frag8(a.f[3]), acc, 4, 4, 3, w.s, 3, a.s);
 }
 
-// Few rows: a workgroup of 8 waves owns MT x NT blocks of 32 x 32 outputs, its waves take the k-groups in turn,
+// Not enough 256 x 256 tiles for the card: a workgroup of 8 waves owns MT x NT blocks of 32 x 32 outputs, its waves take the k-groups in turn,
 // fragments straight from memory (they are in lane order there) one group ahead, and the eight partial sums meet in
 // LDS in a fixed order.  Weight rows sit on the MFMA's M axis, so a lane ends with 4 consecutive columns of one row.
 template <int MT, int NT, int EPI>
-__global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Operand W, Out o, int groups) {
+__global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Operand W, Out o, int groups, unsigned tiles_m) {
     extern __shared__ float4 part[];          // [8 waves][MT * NT * 4 register quads][64 lanes]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long rb0 = (long)blockIdx.x * MT, nb0 = (long)blockIdx.y * NT;
+    // workgroups go to the XCDs in turn: XCD x takes the x-th run of tiles, column by column of the output
+    const unsigned per = gridDim.x / 8, extra = gridDim.x % 8, xcd = blockIdx.x % 8;
+    const unsigned tile = xcd * per + min(xcd, extra) + blockIdx.x / 8;
+    const long rb0 = (long)(tile % tiles_m) * MT, nb0 = (long)(tile / tiles_m) * NT;
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -749,13 +744,13 @@ int ovd_impl_mxfp4_quant(const void* x, int x_is_f32, long ldx, uint8_t* data, u
                 "mxfp4_quant: rows must keep 16-byte alignment (ldx=%ld)", ldx);
     if (M == 0) return 0;
     const int groups = (int)mx_groups(K);
-    const long waves = (long)ceil_div(M, 32) * groups;
-    OVD_REQUIRE((waves + 3) / 4 < (1L << 31), "mxfp4_quant: grid too large");
-    const dim3 grid((unsigned)((waves + 3) / 4)), blk(256);
+    const long blocks = (long)ceil_div(M, 32) * groups;
+    OVD_REQUIRE(blocks < (1L << 24), "mxfp4_quant: grid too large");
+    const dim3 grid((unsigned)blocks), blk(256);
     if (x_is_f32)
-        hipLaunchKernelGGL(mxfp4_quant_kernel<float>, grid, blk, 0, st, (const float*)x, ldx, data, scale, M, K, groups, waves);
+        hipLaunchKernelGGL(mxfp4_quant_kernel<float>, grid, blk, 0, st, (const float*)x, ldx, data, scale, M, K, groups);
     else
-        hipLaunchKernelGGL(mxfp4_quant_kernel<bf16_t>, grid, blk, 0, st, (const bf16_t*)x, ldx, data, scale, M, K, groups, waves);
+        hipLaunchKernelGGL(mxfp4_quant_kernel<bf16_t>, grid, blk, 0, st, (const bf16_t*)x, ldx, data, scale, M, K, groups);
     OVD_CHECK_LAUNCH("mxfp4_quant");
     return 0;
 }
@@ -768,13 +763,13 @@ int ovd_impl_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out,
                 "mxfp4_dequant: rows must keep 16-byte alignment (ldo=%ld)", ldo);
     if (M == 0) return 0;
     const int groups = (int)mx_groups(K);
-    const long waves = (long)ceil_div(M, 32) * groups;
-    OVD_REQUIRE((waves + 3) / 4 < (1L << 31), "mxfp4_dequant: grid too large");
-    const dim3 grid((unsigned)((waves + 3) / 4)), blk(256);
+    const long blocks = (long)ceil_div(M, 32) * groups;
+    OVD_REQUIRE(blocks < (1L << 24), "mxfp4_dequant: grid too large");
+    const dim3 grid((unsigned)blocks), blk(256);
     if (out_is_f32)
-        hipLaunchKernelGGL(mxfp4_dequant_kernel<float>, grid, blk, 0, st, data, scale, (float*)out, ldo, M, K, groups, waves);
+        hipLaunchKernelGGL(mxfp4_dequant_kernel<float>, grid, blk, 0, st, data, scale, (float*)out, ldo, M, K, groups);
     else
-        hipLaunchKernelGGL(mxfp4_dequant_kernel<bf16_t>, grid, blk, 0, st, data, scale, (bf16_t*)out, ldo, M, K, groups, waves);
+        hipLaunchKernelGGL(mxfp4_dequant_kernel<bf16_t>, grid, blk, 0, st, data, scale, (bf16_t*)out, ldo, M, K, groups);
     OVD_CHECK_LAUNCH("mxfp4_dequant");
     return 0;
 }
@@ -871,10 +866,10 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
         static OvdLdsLimit lim;                                                                                \
         if (!lim.ensure(reinterpret_cast<const void*>(&gemm_mxfp4_direct_kernel<MT, NT, E>), lds))             \
             OVD_FAIL("gemm_mxfp4: cannot reserve %zu bytes of LDS", lds);                                      \
-        const int ty = ceil_div(E == EPI_MX_GELU ? ceil_div(N, KG) * KG : N, 32 * NT);                         \
-        OVD_REQUIRE(ty <= 65535, "gemm_mxfp4: grid too large");                                                \
-        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3(ceil_div(M, 32 * MT), ty), dim3(512),   \
-                           lds, st, A, W, o, groups);                                                          \
+        const long tm = ceil_div(M, 32 * MT), tn = ceil_div(E == EPI_MX_GELU ? ceil_div(N, KG) * KG : N, 32 * NT); \
+        OVD_REQUIRE(tm * tn < (1L << 23), "gemm_mxfp4: grid too large");                                       \
+        hipLaunchKernelGGL((gemm_mxfp4_direct_kernel<MT, NT, E>), dim3((unsigned)(tm * tn)), dim3(512),        \
+                           lds, st, A, W, o, groups, (unsigned)tm);                                            \
     }
 #define BIG(E)                                                                                                 \
     {                                                                                                          \
@@ -887,9 +882,18 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
     const int tiles_m = ceil_div(M, TM), tiles_n = ceil_div(N, TN);
     const int cus = max(8, ovd_device_cus() / 8 * 8);
     OVD_REQUIRE((long)tiles_m * tiles_n < (1L << 30), "gemm_mxfp4: grid too large");
-    const bool big = groups >= 2 && (long)tiles_m * tiles_n >= cus / 2;
+    // Which kernel, by the time that its rounds of workgroups take, in units of 0.19 us.  Measured over M 9 .. 2000 at
+    // (N, K) of (1536, 1536), (8960, 1536), (1536, 8960), (5120, 5120), (13824, 5120), (5120, 13824), three operand sets in
+    // turn: a round of 256 x 256 tiles 4.5 + 1.2 groups us, one of 64 x 64 tiles 3.1 + 0.19 groups (550 x 1536 x 8960:
+    // 12 us against 47; 800 x 8960 x 1536: 31 against 15).  32 x 32 tiles, of which several share a CU, take 0.3 rounds of
+    // 64 x 64 ones per tile and CU, and one such time to begin (64 x 1536 x 8960: 5.1 us against 10.2; 550: 15 against 12).
+    const int outs = epilogue == EPI_MX_GELU ? ceil_div(N, KG) * KG : N;
+    const long tiny = (long)ceil_div(M, 32) * ceil_div(outs, 32), small = (long)ceil_div(M, 64) * ceil_div(outs, 64);
+    const long t_big = ceil_div((long)tiles_m * tiles_n, cus) * (23L + 6 * groups);
+    const long t_small = ceil_div(small, cus) * (16L + groups), t_tiny = 3 * (tiny + cus) * (16L + groups) / (10L * cus);
+    const bool big = groups >= 2 && t_big < min(t_small, t_tiny);
     const int wide = (ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) ? 1 : 0;
-#define GEMM_CASE(E) case E: if (big) BIG(E) else if (M <= 32) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
+#define GEMM_CASE(E) case E: if (big) BIG(E) else if (t_tiny < t_small) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
     switch (epilogue) { GEMM_CASE(EPI_BF16) GEMM_CASE(EPI_BF16_GELU) GEMM_CASE(EPI_F32) GEMM_CASE(EPI_RESID) GEMM_CASE(EPI_MX_GELU) }
 #undef GEMM_CASE
 #undef BIG
