@@ -833,7 +833,9 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.stripes = kv_heads % 8 == 0 ? 1 : kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 4 : 8;
     const long per_unit = (p.row_blocks + a.stripes - 1) / a.stripes;
     const long grid = p.split ? (long)p.row_blocks * kv_heads : per_unit * a.stripes * kv_heads;
-    OVD_REQUIRE(grid < (1L << 31), "attn_packed: grid too large");
+    // a launch holds fewer than 2^32 threads
+    OVD_REQUIRE(grid * 64 * p.waves < (1L << 32) && (a.max_splits == 1 || total_q * q_heads < (1L << 24)),
+                "attn_packed: grid too large");
     const size_t lds = 4 * BKV * D * 2;
 #define PACKED(KERNEL, NW)                                                                                      \
     {                                                                                                           \
@@ -860,9 +862,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
 #undef PACKED
     OVD_CHECK_LAUNCH("attn_packed");
     if (p.split && a.max_splits > 1) {
-        const long rows = total_q * q_heads;
-        OVD_REQUIRE(rows < (1L << 31), "attn_packed: grid too large");
-        const dim3 jg((unsigned)rows), jb(256);
+        const dim3 jg((unsigned)(total_q * q_heads)), jb(256);
         if (D == 128) hipLaunchKernelGGL(attn_packed_join_kernel<128>, jg, jb, 0, st, a);
         else hipLaunchKernelGGL(attn_packed_join_kernel<64>, jg, jb, 0, st, a);
         OVD_CHECK_LAUNCH("attn_packed join");

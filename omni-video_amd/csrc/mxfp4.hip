@@ -856,6 +856,7 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
     if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
     OVD_REQUIRE(reinterpret_cast<uintptr_t>(a_data) % 16 == 0 && reinterpret_cast<uintptr_t>(a_scale) % 4 == 0,
                 "gemm_mxfp4: operands must be 16-byte aligned");
+    OVD_REQUIRE(epilogue != EPI_MX_GELU || (out != a_data && out != w_data), "gemm_mxfp4: the output matrix is one of the operands");
     if (M == 0) return 0;
     const Operand A{a_data, a_scale, M}, W{w_data, w_scale, N};
     const Out o{bias, out, ldo, gate};

@@ -145,7 +145,7 @@ int ovd_impl_rope_positions(const void* x, int is_f32, long ldx, const void* pos
     a.heads_per_pass = heads < slots ? heads : slots;
     a.tokens_per_wave = slots / a.heads_per_pass;
     const long blocks = (tokens + 4L * a.tokens_per_wave - 1) / (4L * a.tokens_per_wave);
-    OVD_REQUIRE(blocks < (1L << 31), "rope_positions: grid too large");
+    OVD_REQUIRE(blocks < (1L << 24), "rope_positions: grid too large");
 #define ROPE_LAUNCH(T, P, I)                                                                                \
     hipLaunchKernelGGL((rope_positions_kernel<T, P, I>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)x, \
                        (T*)out, (const P*)pos, a)

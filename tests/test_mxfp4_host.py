@@ -117,6 +117,7 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, None, 1, 8, 32, 5, None, why=b"epilogue")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, p, 1, 8, 32, 4, None, why=b"MXFP4 output")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 32, None, 1, 32, 32, 4, None, why=b"MXFP4 output")
+    refused("ovd_gemm_mxfp4", p, p, p + 16, p, None, p, 32, p, 1, 32, 32, 4, None, why=b"one of the operands")
     refused("ovd_linear_mxfp4", p, 0, 32, p, p, None, p, 32, p, None, 0, 2, 32, 32, 4, None, why=b"quantised x")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 8, p, 1, 8, 32, 0, None, why=b"gate")
     refused("ovd_gemm_mxfp4", p, p, p, p, None, p, 4, None, 1, 8, 32, 0, None, why=b"ldo")

@@ -92,11 +92,12 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_rope_positions", *rope(D=528, ldx=2048, ldo=2048), why=b"head_dim")
     refused("ovd_rope_positions", *rope(axes=9), why=b"axes")
     refused("ovd_rope_positions", *rope(T=-1), why=b"tokens")
+    refused("ovd_rope_positions", *rope(T=2 ** 40), why=b"grid too large")
     refused("ovd_rope_positions", *rope(ldx=60), why=b"alignment")
     refused("ovd_rope_positions", *rope(x=p + 2), why=b"alignment")
 
-    def attn(q=p, k=p, Tq=4, Tk=4, docs=1, mq=4, N=2, Nk=1, D=64, q_ld=128, k_ld=64, causal=0, prefix=None, scale=0.1, cap=0.0):
-        return (q, k, k, p, Tq, Tk, p, p, docs, mq, 4, N, Nk, D, q_ld, k_ld, 64, 128, causal, prefix, scale, cap, None, 0, None)
+    def attn(q=p, k=p, Tq=4, Tk=4, docs=1, mq=4, N=2, Nk=1, D=64, q_ld=128, k_ld=64, v_ld=64, o_ld=128, causal=0, prefix=None, scale=0.1, cap=0.0):
+        return (q, k, k, p, Tq, Tk, p, p, docs, mq, 4, N, Nk, D, q_ld, k_ld, v_ld, o_ld, causal, prefix, scale, cap, None, 0, None)
     refused("ovd_attn_packed_fwd_bf16", *attn(q=None), why=b"null")
     refused("ovd_attn_packed_fwd_bf16", *attn(k=None), why=b"null")
     refused("ovd_attn_packed_fwd_bf16", *attn(D=96), why=b"head_dim")
@@ -110,6 +111,8 @@ def test_c_entries_refuse_before_any_launch():
     refused("ovd_attn_packed_fwd_bf16", *attn(cap=math.nan), why=b"softcap")
     refused("ovd_attn_packed_fwd_bf16", *attn(prefix=p), why=b"prefix")
     refused("ovd_attn_packed_fwd_bf16", *attn(mq=-1), why=b"bound")
+    refused("ovd_attn_packed_fwd_bf16", *attn(docs=2 ** 26), why=b"too many query rows")
+    refused("ovd_attn_packed_fwd_bf16", *attn(docs=2 ** 24, N=8, Nk=8, q_ld=512, k_ld=512, o_ld=512, v_ld=512), why=b"grid too large")
     assert L.ovd_attn_packed_fwd_bf16(*attn(Tq=0)) == 0
 
 
