@@ -206,12 +206,14 @@ __device__ __forceinline__ bf16x8 read_v(const char* sv, int st, int db, int lan
     return __builtin_bit_cast(bf16x8, make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
 }
 
-// scores of a capped tile in units of log2: cap log2(e) tanh(s scale / cap), tanh(x) = 1 - 2 / (1 + e^2x) (both ends
+// a capped score in units of log2, minus `minus`: cap log2(e) tanh(s scale / cap), tanh(x) = 1 - 2 / (1 + e^2x) (both ends
 // saturate without overflow)
-__device__ __forceinline__ void cap_scores(f32x16& s, float cap_in, float cap_out) {
+__device__ __forceinline__ float capped(float s, const Args& a, float minus) {
+    return __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.cap_in)), a.cap_out - minus);
+}
+__device__ __forceinline__ void cap_scores(f32x16& s, const Args& a) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-        s[j] = __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * cap_in)), cap_out);
+    for (int j = 0; j < 16; ++j) s[j] = capped(s[j], a, 0.f);
 }
 
 __device__ __forceinline__ void mask_scores(f32x16& s0, f32x16& s1, int key0, int nvis, int hi) {
@@ -266,8 +268,8 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
         s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], s1, 0, 0, 0);
     }
     if (CAP) {
-        cap_scores(s0, a.cap_in, a.cap_out);
-        cap_scores(s1, a.cap_in, a.cap_out);
+        cap_scores(s0, a);
+        cap_scores(s1, a);
     }
     mask_scores(s0, s1, t * BKV, nvis, hi);
     const float sc = CAP ? 1.f : a.scale_log2;
@@ -329,7 +331,11 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
 // forms S^T of tile t + 1 in n0 / n1.  K of tile t + 2 and V of tile t + 1 are put in flight from inside.
 // The running maximum m_c is raised only when a tile exceeds it by RESCALE_THR (log2 units): probabilities stay below
 // 2^THR, which costs no relative precision, and most tiles skip the rescale of O.
-template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT>
+// RAW (capped form): tile t's scores are not capped yet.  The cap is monotonic, so the running maximum needs it for one
+// value of a row, and the rest pass through it between this step's products, on their way into the exponential (packed
+// prompts with a cap 62 us; as a pass of its own between the two products 66 us).  Masked scores
+// must not pass through it: such tiles are capped first, then masked.
+template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT, bool RAW>
 __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
                                           const f32x16& c0, const f32x16& c1, f32x16& n0, f32x16& n1, float& mx, bool& need,
                                           const char* sk_next, const char* sv_cur, const Stream<D, NW, true>& kst, char* k_dst,
@@ -355,12 +361,13 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
     const float sc = CAP ? 1.f : a.scale_log2;
     float rs0 = 0.f, rs1 = 0.f;
     uint32_t pw[16];
+#define EXPONENT(x) (RAW ? capped(x, a, m_c) : CAP ? (x) - m_c : __builtin_fmaf(x, sc, -m_c))
 #define SOFTMAX_PAIR(i)                                                                                    \
     do {                                                                                                   \
         const f32x16& c_ = (i) < 8 ? c0 : c1;                                                              \
         const int r_ = ((i) & 7) * 2;                                                                      \
-        const float pa_ = __builtin_amdgcn_exp2f(CAP ? c_[r_] - m_c : __builtin_fmaf(c_[r_], sc, -m_c));   \
-        const float pb_ = __builtin_amdgcn_exp2f(CAP ? c_[r_ + 1] - m_c : __builtin_fmaf(c_[r_ + 1], sc, -m_c)); \
+        const float pa_ = __builtin_amdgcn_exp2f(EXPONENT(c_[r_]));                                        \
+        const float pb_ = __builtin_amdgcn_exp2f(EXPONENT(c_[r_ + 1]));                                    \
         rs0 += pa_;                                                                                        \
         rs1 += pb_;                                                                                        \
         pw[i] = pack_bf2(pa_, pb_);                                                                        \
@@ -395,13 +402,12 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (HAS_NEXT && CAP) {
-        cap_scores(n0, a.cap_in, a.cap_out);
-        cap_scores(n1, a.cap_in, a.cap_out);
+    if (HAS_NEXT && MASK_NEXT && CAP) {
+        cap_scores(n0, a);
+        cap_scores(n1, a);
     }
     if (HAS_NEXT && MASK_NEXT) mask_scores(n0, n1, (t + 1) * BKV, nvis, hi);
     float nmx = -3.0e38f;
-    const float sc_next = CAP ? 1.f : a.scale_log2;
     if ((MASK_NEXT || !HAS_NEXT) && masked_cur) redo |= tile_not_finite<D>(sv_cur, lane);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -423,7 +429,7 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
             for (int r = 0; r < 16; r += 2) nmx = max3(nmx, n[r], n[r + 1]);
             asm volatile("" : "+v"(nmx));
             if (st == 3) {
-                mx = half_max(nmx) * sc_next;
+                mx = CAP ? (MASK_NEXT ? half_max(nmx) : capped(half_max(nmx), a, 0.f)) : half_max(nmx) * a.scale_log2;
                 need = __any(mx > m_c + RESCALE_THR);
             }
         }
@@ -431,6 +437,7 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
     }
     l_run += rs0 + rs1;
 #undef SOFTMAX_PAIR
+#undef EXPONENT
 }
 
 // one work item: 32 NW rows of document `doc` under key head kvh, part `part` of `parts` of their keys
@@ -503,15 +510,17 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
                 a0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf0, qf[ks], a0, 0, 0, 0);
                 a1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], a1, 0, 0, 0);
             }
-            if (CAP) {
-                cap_scores(a0, a.cap_in, a.cap_out);
-                cap_scores(a1, a.cap_in, a.cap_out);
+            if (t0 >= tf) {
+                if (CAP) {
+                    cap_scores(a0, a);
+                    cap_scores(a1, a);
+                }
+                mask_scores(a0, a1, t0 * BKV, nvis, hi);
             }
-            if (t0 >= tf) mask_scores(a0, a1, t0 * BKV, nvis, hi);
             float nmx = -3.0e38f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) nmx = max3(nmx, a0[r], a1[r]);
-            mx = half_max(nmx) * (CAP ? 1.f : a.scale_log2);
+            mx = CAP ? (t0 < tf ? capped(half_max(nmx), a, 0.f) : half_max(nmx)) : half_max(nmx) * a.scale_log2;
             need = __any(mx > m_c + RESCALE_THR);
         }
         __syncthreads();      // every wave is done with K(t0) before K(t0 + 2) overwrites it
@@ -519,7 +528,8 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
 #define PIPE_STEP(HAS_NEXT, MASK_NEXT, C0, C1, N0, N1, U)                                                           \
     do {                                                                                                            \
         const int u_ = (U), t_ = t0 + u_;                                                                           \
-        pipe_step<D, NW, CAP, HAS_NEXT, MASK_NEXT>(o_acc, qf, m_c, l_run, C0, C1, N0, N1, mx, need,                 \
+        pipe_step<D, NW, CAP, HAS_NEXT, MASK_NEXT, CAP && HAS_NEXT && !MASK_NEXT>(                                  \
+            o_acc, qf, m_c, l_run, C0, C1, N0, N1, mx, need,                                                        \
                                                    smem + ((u_ + 1) & 1) * TILE, smem + (2 + (u_ & 1)) * TILE, kst, \
                                                    smem + (u_ & 1) * TILE, t_ + 2 < t1, vst,                        \
                                                    smem + (2 + ((u_ + 1) & 1)) * TILE, t_ + 1 < t1, t_, nvis,       \
@@ -537,6 +547,10 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
             a0 = b0;
             a1 = b1;
             ++u;
+        }
+        if (CAP && t0 < tf) {                 // the last whole tile
+            cap_scores(a0, a);
+            cap_scores(a1, a);
         }
         for (; t0 + u + 1 < tw; ++u) {
             PIPE_STEP(true, true, a0, a1, b0, b1, u);
