@@ -21,6 +21,12 @@
 // from the row-major V tile through ds_read_b64_tr_b16; K and V tiles of 64 keys stream HBM -> LDS by DMA with the
 // bank swizzle applied to the source chunk.  Key rows past the document are clamped to its last row: what lies behind
 // a document is never read, and a masked score is -inf whatever it was.
+//
+// What bounds it.  D = 128, long documents: the matrix pipe and the chip's power (20280, 1560, 14040 and 3600 tokens, 40
+// heads: 10.8 ms = 1180 TFLOP/s; one document of 20280 as fast as attn.hip).  D = 64: vector instructions (197 a tile and
+// wave beside 16 matrix ones: 970 TFLOP/s), the more so with a cap (two transcendental instructions a score: 500).  Few
+// tokens: bytes of K and V (8 tokens against 80150 keys, 8 key heads: 76 us with the join = 4.4 TB/s).  Prompts of
+// some hundred tokens: the start and the last, partly filled round (8 of them, 16 heads of 64, a prefix: 47 us, 62 capped).
 #include "common.h"
 
 namespace {
@@ -82,7 +88,7 @@ __device__ __forceinline__ int parts_of(const Args& a, int lk) {
 
 // document, row block (of ROWS rows) and part of its keys of work item `blk`; false past the last one.  Up to SORTED
 // documents are walked from the longest keys to the shortest, so that the last workgroups to start are short ones (packed
-// prompts of 1 to 2100 tokens, 4 key heads: 92 us in the order given, 77 sorted); more are taken in their order.
+// prompts of 1 to 2100 tokens, 4 key heads, with eight-wave workgroups: 92 us in the order given, 77 sorted); more are taken in their order.
 constexpr int SORTED = 32;
 
 template <int ROWS, bool SPLIT>
@@ -333,8 +339,9 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
 // 2^THR, which costs no relative precision, and most tiles skip the rescale of O.
 // RAW (capped form): tile t's scores are not capped yet.  The cap is monotonic, so the running maximum needs it for one
 // value of a row, and the rest pass through it between this step's products, on their way into the exponential (packed
-// prompts with a cap 62 us; as a pass of its own between the two products 66 us).  Masked scores
-// must not pass through it: such tiles are capped first, then masked.
+// prompts with a cap 62 us; as a pass of its own between the two products 66 us).  Masked scores must not pass through it:
+// such tiles are capped first, then masked.  Three buffers of K and V instead of two: D = 64 10 % slower (the
+// buffers' addresses cost vector instructions; the loads are in time).
 template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT, bool RAW>
 __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
                                           const f32x16& c0, const f32x16& c1, f32x16& n0, f32x16& n1, float& mx, bool& need,
@@ -738,7 +745,8 @@ struct Plan {
 // V half as often and are 7 % faster in full rounds, but a last round that is partly filled costs them a whole one.
 //   short keys: four (60 documents of 257 tokens, 12 heads: 80 us against 98);
 //   causal (lengths differ, longest first): four below three rounds of eight (packed prompts of 1 to 2100 tokens with a cap
-//   68 us against 77; 6000 tokens, 12 heads 134 against 143; 20280 tokens, 12 heads: 1239 against 1188);
+//   68 us against 77, the cap being a pass of its own then; 6000 tokens, 12 heads 134 against 143; 20280 tokens, 12 heads:
+//   1239 against 1188);
 //   otherwise by rounds, a round of four-wave workgroups that run alone on their CUs counted as 0.6 (6000 tokens, 12
 //   heads: 274 us against 297; three documents of 3000: 183 against 166; 20280: 2331 against 2151).
 bool wide_workgroups(long rows, int docs, int kv_heads, int causal, long max_k, long cus) {
@@ -766,7 +774,7 @@ Plan plan_of(long total_q, long total_k, int docs, int kv_heads, int group, int 
         // All parts have about the same number of tiles, `chunk`, and `slots` workgroups run at a time.  R rounds leave
         // R slots - (one partly filled part per row block) parts for the tiles; a workgroup's start costs about as much
         // as 4 tiles.  The number of rounds that this puts first (8 tokens against 1 to 32760 keys, 8 key heads: one
-        // round of 23 tiles 69 us, four rounds of 5 tiles 88 us).
+        // round of 23 tiles 70 us before the join, four rounds of 5 tiles 88 us).
         const long most = (max_k + BKV - 1) / BKV;
         long tiles = p.waves == 1 ? total_k / BKV + docs : most * p.row_blocks;
         if (tiles > most * p.row_blocks) tiles = most * p.row_blocks;

@@ -56,7 +56,8 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 // ------------------------------------------------------------------------------------------ quantise / dequantise
 // One workgroup = one row block x one k-group, a wave 8 of its rows.  A load instruction covers 8 rows x 64 k (8 lanes of
 // 8 values per row: whole 128-byte lines of bf16), a store instruction two runs of 8 rows x 16 bytes; the four lanes of an
-// MX block exchange their largest magnitude.  HBM-bound: 2 (4) bytes read and 17/32 written per value.
+// MX block exchange their largest magnitude.  HBM-bound: 2 (4) bytes read and 17/32 written per value: 40560 x 8960 bf16
+// 165 us = 5.6 TB/s, back in 160 us (a wave over all 32 rows of the block: 186 and 180, and 550 x 8960 11.5 us instead of 4.3).
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
 template <>
@@ -277,9 +278,11 @@ __device__ __forceinline__ void mfma_group(f32x16& acc, const Group& w, const Gr
     acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.f[3]), frag8(a.f[3]), acc, 4, 4, 3, w.s, 3, a.s);
 }
 
-// Not enough 256 x 256 tiles for the card: a workgroup of 8 waves owns MT x NT blocks of 32 x 32 outputs, its waves take the k-groups in turn,
-// fragments straight from memory (they are in lane order there) one group ahead, and the eight partial sums meet in
-// LDS in a fixed order.  Weight rows sit on the MFMA's M axis, so a lane ends with 4 consecutive columns of one row.
+// Not enough 256 x 256 tiles for the card: a workgroup of 8 waves owns MT x NT blocks of 32 x 32 outputs, its waves take
+// the k-groups in turn, fragments straight from memory (they are in lane order there) one group ahead, and the eight
+// partial sums meet in LDS in a fixed order.  Weight rows sit on the MFMA's M axis, so a lane ends with 4 consecutive
+// columns of one row.  Bound by the trips to memory (4 to 5 a wave at K = 8960) and the traffic of L2: 550 x 1536 x 8960
+// 12 us = 1.3 PFLOP/s (tiles in the order of the workgroups instead of runs per XCD: 15 us).
 template <int MT, int NT, int EPI>
 __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Operand W, Out o, int groups, unsigned tiles_m) {
     extern __shared__ float4 part[];          // [8 waves][MT * NT * 4 register quads][64 lanes]
@@ -379,7 +382,8 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
 
 // A handful of rows (M <= FEW_ROWS) straight from bf16 / fp32: every workgroup quantises all of x into LDS (a few thousand
 // values) under its first weight loads, so a token's layer is one launch.  A workgroup owns one block of 32 weight rows;
-// its waves take the k-groups in turn and meet as above.  LDS: codes [group][ks][h][FEW_ROWS][16], scales
+// its waves take the k-groups in turn and meet as above.  Bound by the weights: one row of 5120 x 5120 5.4 us (launch
+// and one trip to memory 3, 13.9 MB of weights the rest); as two launches 8.  LDS: codes [group][ks][h][FEW_ROWS][16], scales
 // [group][h][FEW_ROWS][4], then the partial sums.
 constexpr int FEW_ROWS = 8;
 constexpr int FEW_GRP = 8 * FEW_ROWS * 16 + 2 * FEW_ROWS * 4;       // LDS bytes per k-group
@@ -456,6 +460,11 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
 // The tile layout makes every DMA instruction 1 KiB of consecutive memory and every fragment read 1 KiB of consecutive
 // LDS: no swizzle.  Scales travel the same way, one 256-byte instruction per row block and K-tile (8 KiB of LDS for two
 // buffers); they are issued with phase 4, so any four consecutive phases hold 10 DMA instructions of a wave.
+// 32760 x 5120 x 13824: 1.0 ms = 4.6 PFLOP/s, bound by power: the matrix pipe is busy 62 % of cycles at the 1.43 GHz that
+// the chip then holds, and operands of zeros run 25 % faster.  40560 x 8960 x 1536: 345 us bf16, 400 with GELU, 380 to 430
+// with the GELU quantised: with six k-groups a tile the epilogue is a third of the time (its vector work and the stores).
+// Not better: four waves of 128 x 128 outputs (4.3 PFLOP/s, a longer epilogue); 128 x 256 tiles in two workgroups per CU
+// (long K 3.8 PFLOP/s; short K with GELU 406 us against 421 then).
 constexpr int TM = 256, TN = 256;
 constexpr int PBUF = 2 * 8 * GRP_DATA;            // one buffer: A 8 row blocks x 4 KiB | W the same
 constexpr int SBUF = 2 * 8 * GRP_SCALE;           // its scales

@@ -9,7 +9,8 @@
 // The angle is a 64-bit product reduced to a quarter turn in 64 bits, then sine and cosine by their Taylor polynomials in
 // 32 bits (|r| <= pi/4: truncation below 2e-9): positions of any size cost no accuracy and there is no table to outgrow.
 // HBM-bound (every element read and written once): a lane owns 8 (bf16, fp32 alike) values of a head, computes the
-// turns of its pairs once per token and applies them to every head of the token that falls to it.
+// turns of its pairs once per token and applies them to every head of the token that falls to it.  56640 tokens x 12 heads
+// of 128, bf16: 65 us = 5.3 TB/s.
 #include "common.h"
 
 namespace {
