@@ -242,6 +242,33 @@ __device__ __forceinline__ uint32_t store_mx(const Out& o, const f32x16& acc, co
     }
     return s;
 }
+// The same for a wave that holds 16 rows x 32 columns of a block in two 16 x 16 pieces (register j of y0 / y1 of lane l: row
+// l & 15, column 4 (l >> 4) + j / 16 + that): a row lies in four lanes, each of which ends up with four bytes of its codes
+// and writes them to `row_codes`, the row's 16 bytes.
+__device__ __forceinline__ uint32_t pack_mx16(const f32x4& y0, const f32x4& y1, const uint2 (&bias)[2], bool inside, char* row_codes,
+                                              int lane) {
+    float t0[4] = {y0[0], y0[1], y0[2], y0[3]}, t1[4] = {y1[0], y1[1], y1[2], y1[3]};
+    add_bias(t0, bias[0]);
+    add_bias(t1, bias[1]);
+    float y[8];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = inside ? gelu_tanh_f(i < 4 ? t0[i & 3] : t1[i & 3]) : 0.f;
+        mx = umax(mx, __float_as_uint(y[i]) & 0x7fffffffu);
+    }
+    const auto e0 = __builtin_amdgcn_permlane16_swap(mx, mx, false, false);
+    mx = umax(e0[0], e0[1]);
+    const auto e1 = __builtin_amdgcn_permlane32_swap(mx, mx, false, false);
+    const uint32_t s = scale_byte(umax(e1[0], e1[1]));
+    // columns 4 q .. 4 q + 3 in the low half of lane quarter q's word, 16 columns on in the high half: even quarters take the
+    // low halves of a pair, odd ones the high halves
+    const uint32_t c = pack_fp4x8(y, cvt_scale(s));
+    const auto ex = __builtin_amdgcn_permlane16_swap(c, c >> 16, false, false);
+    const int q = lane >> 4;
+    *reinterpret_cast<uint32_t*>(row_codes + (q & 1) * 8 + (q >> 1) * 4) = (ex[0] & 0xffffu) | (ex[1] << 16);
+    return s;
+}
 // the scale buffer of an MXFP4 output (o.gate holds its address)
 __device__ __forceinline__ uint8_t* mx_scales(const Out& o) { return reinterpret_cast<uint8_t*>(const_cast<float*>(o.gate)); }
 
@@ -455,16 +482,20 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
 // ------------------------------------------------------------------------------------------ product, many rows
 // The four-phase schedule of gemm256.hip on 256 x 256 output tiles: K-tiles of one k-group (128 bytes of codes per row,
 // 64 KiB for both operands), two LDS buffers, one 16 KiB half-tile staged per phase, DMA never drained inside the loop,
-// the two wave groups one barrier apart.  A phase is 8 v_mfma_scale_f32_32x32x64_f8f6f4 on fp4 operands: the matrix time
+// the two wave groups one barrier apart.  A phase is 16 v_mfma_scale_f32_16x16x128_f8f6f4 on fp4 operands: the matrix time
 // of the 4 e4m3 ones of fp8.hip's phase for twice the K, so LDS and DMA bytes per matrix cycle are the same.
-// The tile layout makes every DMA instruction 1 KiB of consecutive memory and every fragment read 1 KiB of consecutive
+// The tile layout makes every DMA instruction 1 KiB of consecutive memory and every fragment read four runs of 256 bytes of
 // LDS: no swizzle.  Scales travel the same way, one 256-byte instruction per row block and K-tile (8 KiB of LDS for two
 // buffers); they are issued with phase 4, so any four consecutive phases hold 10 DMA instructions of a wave.
-// 32760 x 5120 x 13824: 1.0 ms = 4.6 PFLOP/s, bound by power: the matrix pipe is busy 62 % of cycles at the 1.43 GHz that
-// the chip then holds, and operands of zeros run 25 % faster.  40560 x 8960 x 1536: 345 us bf16, 400 with GELU, 380 to 430
-// with the GELU quantised: with six k-groups a tile the epilogue is a third of the time (its vector work and the stores).
+// 32760 x 5120 x 13824: 0.97 ms = 4.8 PFLOP/s, bound by power: the matrix pipe is busy 60 % of cycles at the 1.4 to 1.7 GHz
+// that the chip then holds, and operands of zeros run 25 % faster.  The instruction shape is a matter of power, too: a loop
+// of products of Gaussian values alone holds 6.8 PFLOP/s as 32x32x64, 7.4 as 16x16x128 (fewer accumulators pass by per
+// product), 7.55 where only one operand changes from one to the next; the whole product gains 2 to 4 %.
+// 40560 x 8960 x 1536: 337 us bf16, 403 with GELU, 440 with the GELU quantised: with six k-groups a tile the epilogue is a
+// third of the time (its vector work and the stores).
 // Not better: four waves of 128 x 128 outputs (4.3 PFLOP/s, a longer epilogue); 128 x 256 tiles in two workgroups per CU
-// (long K 3.8 PFLOP/s; short K with GELU 406 us against 421 then).
+// (long K 3.8 PFLOP/s; short K with GELU 406 us against 421 then); the closing barriers ahead of a phase's last products
+// (2000 x 5120 x 5120 36.5 us against 34: the next reads wait behind them).
 constexpr int TM = 256, TN = 256;
 constexpr int PBUF = 2 * 8 * GRP_DATA;            // one buffer: A 8 row blocks x 4 KiB | W the same
 constexpr int SBUF = 2 * 8 * GRP_SCALE;           // its scales
@@ -505,28 +536,48 @@ __device__ __forceinline__ void phase_close() {
 }
 
 struct Frag4 {
-    i32x4 k[4];                  // a row block's four k-steps
+    i32x4 f[2][2];               // a row block: its two halves of 16 rows, two k-steps of 128
 };
 __device__ __forceinline__ i32x8 frag8(const i32x4& u) { return (i32x8){u[0], u[1], u[2], u[3], 0, 0, 0, 0}; }
-__device__ __forceinline__ Frag4 lds_frags(const char* p, int lane) {
-    Frag4 f;
+__device__ __forceinline__ Frag4 lds_frags(const char* p) {
+    Frag4 r;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) f.k[ks] = *reinterpret_cast<const i32x4*>(p + ks * FRAG + lane * 16);
-    return f;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) r.f[i][s] = *reinterpret_cast<const i32x4*>(p + s * 2 * FRAG + i * 256);
+    return r;
 }
 
-#define MX_STEP(KS)                                                                                                       \
-    a0 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.k[KS]), frag8(x[0].k[KS]), a0, 4, 4, KS, ws, KS, xs0);   \
-    a1 = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag8(w.k[KS]), frag8(x[1].k[KS]), a1, 4, 4, KS, ws, KS, xs1);
-__device__ __forceinline__ void quadrant(f32x16& a0, f32x16& a1, const Frag4& w, int ws, const Frag4 (&x)[2], int xs0, int xs1) {
-    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+// scales of N 16-row groups.  A lane's dword holds the bytes of k-blocks h, h + 2, h + 4, h + 6 (h = its quarter & 1): shifted by
+// its quarter / 2 bytes, bytes 0 and 2 are those of its blocks in the two k-steps
+template <int N>
+__device__ __forceinline__ void read_scales(int (&s)[N], const char* p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = *reinterpret_cast<const int*>(p + (i >> 1) * GRP_SCALE + (i & 1) * 64);
+}
+template <int N>
+__device__ __forceinline__ void shift_scales(int (&s)[N], int shift) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = (unsigned)s[i] >> shift;
+}
+
+// 32 columns x 64 rows x 256 k.  From product to product only one operand changes: 2 % more than in plain order
+#define MX_MFMA(J, I, S)                                                                                                     \
+    c[J][I] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(frag8(w.f[J][S]), frag8(x[(I) >> 1].f[(I) & 1][S]), c[J][I], 4, 4, \
+                                                               2 * (S), ws[J], 2 * (S), xs[I]);
+#define MX_STEP(S)                                                                                                           \
+    MX_MFMA(0, 0, S) MX_MFMA(1, 0, S) MX_MFMA(1, 1, S) MX_MFMA(0, 1, S)                                                      \
+    MX_MFMA(0, 2, S) MX_MFMA(1, 2, S) MX_MFMA(1, 3, S) MX_MFMA(0, 3, S)
+__device__ __forceinline__ void quadrant(f32x4 (&c)[2][4], const Frag4& w, const int (&ws)[2], const Frag4 (&x)[2], const int (&xs)[4]) {
+    MX_STEP(0) MX_STEP(1)
 }
 #undef MX_STEP
+#undef MX_MFMA
 
 // TAIL 0: steady state, 1: next-to-last K-tile, 2: last
 template <int TAIL>
-__device__ __forceinline__ void k_tile(f32x16 (&acc)[2][4], char* smem, int buf, long kg1, long kg2, const Feed& fa, const Feed& fw,
-                                       int a_rd, int w_rd, int sa_rd, int sw_rd, int wave, int lane) {
+__device__ __forceinline__ void k_tile(f32x4 (&acc)[2][2][2][4], char* smem, int buf, long kg1, long kg2, const Feed& fa, const Feed& fw,
+                                       int a_rd, int w_rd, int sa_rd, int sw_rd, int wave, int shift) {
     const char* ca = smem + buf * PBUF + a_rd;
     const char* cw = smem + buf * PBUF + PBUF / 2 + w_rd;
     char* own = smem + buf * PBUF + wave * 1024;
@@ -534,31 +585,34 @@ __device__ __forceinline__ void k_tile(f32x16 (&acc)[2][4], char* smem, int buf,
     char* sbuf = smem + 2 * PBUF + buf * SBUF;
     Frag4 w0, w1, af[2];
     // phase 1
-    w0 = lds_frags(cw, lane);
-    af[0] = lds_frags(ca, lane);
-    af[1] = lds_frags(ca + GRP_DATA, lane);
-    int xs[4], ws[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        xs[i] = *reinterpret_cast<const int*>(sbuf + ((i >> 1) * 4 + (i & 1)) * GRP_SCALE + sa_rd);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ws[i] = *reinterpret_cast<const int*>(sbuf + (8 + i * 4) * GRP_SCALE + sw_rd);
+    w0 = lds_frags(cw);
+    af[0] = lds_frags(ca);
+    af[1] = lds_frags(ca + GRP_DATA);
+    int xs[4], ws0[2], ws1[2];
+    read_scales(xs, sbuf + sa_rd);
+    read_scales(ws0, sbuf + 8 * GRP_SCALE + sw_rd);
     if (TAIL < 2) stage_half<1>(fw, kg1, oth + PBUF / 2);
     phase_open<TAIL == 2 ? 2 : 10>();
-    quadrant(acc[0][0], acc[0][1], w0, ws[0], af, xs[0], xs[1]);
+    shift_scales(xs, shift);
+    shift_scales(ws0, shift);
+    quadrant(acc[0][0], w0, ws0, af, xs);
     phase_close();
     // phase 2
-    w1 = lds_frags(cw + 4 * GRP_DATA, lane);
+    w1 = lds_frags(cw + 4 * GRP_DATA);
+    read_scales(ws1, sbuf + 12 * GRP_SCALE + sw_rd);
     if (TAIL < 2) stage_half<1>(fa, kg1, oth);
     phase_open<TAIL == 2 ? 0 : 10>();
-    quadrant(acc[1][0], acc[1][1], w1, ws[1], af, xs[0], xs[1]);
+    shift_scales(ws1, shift);
+    quadrant(acc[1][0], w1, ws1, af, xs);
     phase_close();
     // phase 3
-    af[0] = lds_frags(ca + 4 * GRP_DATA, lane);
-    af[1] = lds_frags(ca + 5 * GRP_DATA, lane);
+    af[0] = lds_frags(ca + 4 * GRP_DATA);
+    af[1] = lds_frags(ca + 5 * GRP_DATA);
+    read_scales(xs, sbuf + 4 * GRP_SCALE + sa_rd);
     if (TAIL == 0) stage_half<0>(fw, kg2, own + PBUF / 2);
     phase_open<-1>();
-    quadrant(acc[1][2], acc[1][3], w1, ws[1], af, xs[2], xs[3]);
+    shift_scales(xs, shift);
+    quadrant(acc[1][1], w1, ws1, af, xs);
     phase_close();
     // phase 4
     if (TAIL == 0) {
@@ -566,12 +620,12 @@ __device__ __forceinline__ void k_tile(f32x16 (&acc)[2][4], char* smem, int buf,
         stage_scales(fa, fw, kg2, sbuf + wave * GRP_SCALE);
     }
     phase_open<TAIL == 0 ? 10 : TAIL == 1 ? 4 : -1>();
-    quadrant(acc[0][2], acc[0][3], w0, ws[0], af, xs[2], xs[3]);
+    quadrant(acc[0][1], w0, ws0, af, xs);
     if (TAIL != 0) {
         // a use in front of the closing barrier: the MFMAs of the last K-tiles would otherwise sink past it
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
+        for (int i = 0; i < 16; ++i)
+            asm volatile("" : "+v"(acc[i >> 3][(i >> 2) & 1][0][i & 3]), "+v"(acc[i >> 3][(i >> 2) & 1][1][i & 3]));
     }
     phase_close();
 }
@@ -604,28 +658,28 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
         fa.scale = A.scale + (long)min(tm * 8 + wave, a_last) * groups * GRP_SCALE + lane * 4;
         fw.scale = W.scale + (long)min(tn * 8 + wave, w_last) * groups * GRP_SCALE + lane * 4;
     }
-    const int a_rd = wr * 2 * GRP_DATA, w_rd = wc * GRP_DATA;
-    const int sa_rd = wr * 2 * GRP_SCALE + lane * 4, sw_rd = wc * GRP_SCALE + lane * 4;
-    uint2 bias[2][4];                    // loaded ahead of the DMA: no ordinary load waits behind it
+    // operand lanes of v_mfma_scale_f32_16x16x128: row l & 15, k-block quarter l >> 4 of a step of 128; in the layout, block
+    // quarter q is half q & 1 of fragment q >> 1
+    const int fr = lane & 15, quarter = lane >> 4;
+    const int frag_at = (quarter >> 1) * FRAG + (quarter & 1) * 512 + fr * 16, scale_at = (quarter & 1) * 128 + fr * 4;
+    const int a_rd = wr * 2 * GRP_DATA + frag_at, w_rd = wc * GRP_DATA + frag_at, shift = (quarter >> 1) * 8;
+    const int sa_rd = wr * 2 * GRP_SCALE + scale_at, sw_rd = wc * GRP_SCALE + scale_at;
+    uint2 bias[2][2];                    // loaded ahead of the DMA: no ordinary load waits behind it
     if (o.bias) {
 #pragma unroll
         for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                bias[nh][g] = *reinterpret_cast<const uint2*>(o.bias + min(col0 + nh * 128 + wc * 32 + 8 * g + 4 * (lane >> 5), W.rows - 4));
+            for (int g = 0; g < 2; ++g)
+                bias[nh][g] = *reinterpret_cast<const uint2*>(o.bias + min(col0 + nh * 128 + wc * 32 + 16 * g + 4 * quarter, W.rows - 4));
     } else {
 #pragma unroll
         for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) bias[nh][g] = make_uint2(0, 0);
+            for (int g = 0; g < 2; ++g) bias[nh][g] = make_uint2(0, 0);
     }
-    f32x16 acc[2][4];
+    f32x4 acc[2][2][2][4];               // [column half][row half][16 columns][16 rows]
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int i = 0; i < 32; ++i) acc[i >> 4][(i >> 3) & 1][(i >> 2) & 1][i & 3] = (f32x4){0.f, 0.f, 0.f, 0.f};
     char* const wd = smem + wave * 1024;
     char* const sd = smem + 2 * PBUF + wave * GRP_SCALE;
     stage_half<0>(fw, 0, wd + PBUF / 2);
@@ -641,52 +695,56 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
     if (wr == 1) __builtin_amdgcn_s_barrier();            // second half of the waves: one barrier behind
     int t = 0;
     for (; t + 2 < groups; ++t)
-        k_tile<0>(acc, smem, t & 1, t + 1, t + 2, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
-    k_tile<1>(acc, smem, t & 1, t + 1, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
+        k_tile<0>(acc, smem, t & 1, t + 1, t + 2, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, shift);
+    k_tile<1>(acc, smem, t & 1, t + 1, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, shift);
     ++t;
-    k_tile<2>(acc, smem, t & 1, 0, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, lane);
+    k_tile<2>(acc, smem, t & 1, 0, 0, fa, fw, a_rd, w_rd, sa_rd, sw_rd, wave, shift);
     if (wr == 0) __builtin_amdgcn_s_barrier();            // balances the extra barrier above
     asm volatile("" ::: "memory");
 
-    // acc[nh][mh * 2 + mb] register 4 g + j is out[m][n + j], m = row0 + mh * 128 + wr * 64 + mb * 32 + (lane & 31),
-    // n = col0 + nh * 128 + wc * 32 + 8 g + 4 (lane >> 5).  bf16 rows go through LDS (256 rows of 512 bytes, chunk c of row r
+    // acc[nh][mh][g][i] register j is out[m][n + j], m = row0 + mh * 128 + wr * 64 + i * 16 + (lane & 15),
+    // n = col0 + nh * 128 + wc * 32 + 16 g + 4 (lane >> 4).  bf16 rows go through LDS (256 rows of 512 bytes, chunk c of row r
     // at c ^ (r & 15)) so that 32 lanes store one 512-byte row segment.
     constexpr bool NARROW = EPI == EPI_BF16 || EPI == EPI_BF16_GELU;
-    const int fr = lane & 31, fh = lane >> 5;
     if constexpr (EPI == EPI_MX_GELU) {          // a tile's 256 columns are one k-group of the next operand
-        // (the scale bytes of a row's group come from four waves: they meet in LDS, [row block][lane][4] as in memory)
+        // codes and scale bytes meet in LDS, [row block][4 KiB] and [row block][lane][4] as in memory; a wave stores a row block
         const int out_groups = (W.rows + KG - 1) / KG;
+        char* const scales = smem + 8 * GRP_DATA;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 8; ++q)              // mh * 4 + i
 #pragma unroll
             for (int nh = 0; nh < 2; ++nh) {
-                const int rbl = (q >> 1) * 4 + wr * 2 + (q & 1);
-                const long rb = tm * 8 + rbl;
-                const uint32_t sb = store_mx(o, acc[nh][q], bias[nh], rb, tn * 8 + nh * 4 + wc, rb * 32 + fr, A.rows, W.rows, out_groups,
-                                             lane);
-                if (fh == 0) smem[rbl * GRP_SCALE + ((wc & 1) * 32 + fr) * 4 + nh * 2 + (wc >> 1)] = (char)sb;
+                const int rbl = (q >> 2) * 4 + wr * 2 + ((q >> 1) & 1), r = (wc & 1) * 32 + (q & 1) * 16 + fr, ks = nh * 2 + (wc >> 1);
+                const uint32_t sb = pack_mx16(acc[nh][q >> 2][0][q & 3], acc[nh][q >> 2][1][q & 3], bias[nh],
+                                              col0 + nh * 128 + wc * 32 < W.rows, smem + rbl * GRP_DATA + ks * FRAG + r * 16, lane);
+                if (quarter == 0) scales[rbl * GRP_SCALE + r * 4 + ks] = (char)sb;
             }
         __syncthreads();
         const long rb = tm * 8 + wave;
-        if (rb * 32 + fr < A.rows)
+        if (rb * 32 + (lane & 31) < A.rows) {
+            u32x4* data = reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(o.out) + (rb * out_groups + tn) * GRP_DATA) + lane;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                data[ks * 64] = *reinterpret_cast<const u32x4*>(smem + wave * GRP_DATA + ks * FRAG + lane * 16);
             reinterpret_cast<uint32_t*>(mx_scales(o) + (rb * out_groups + tn) * GRP_SCALE)[lane] =
-                reinterpret_cast<const uint32_t*>(smem + wave * GRP_SCALE)[lane];
+                reinterpret_cast<const uint32_t*>(scales + wave * GRP_SCALE)[lane];
+        }
     } else if (NARROW && wide) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)              // mh * 2 + mb
+        for (int q = 0; q < 8; ++q)              // mh * 4 + i
 #pragma unroll
             for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x16& a16 = acc[nh][q];
-                    float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
+                for (int g = 0; g < 2; ++g) {
+                    const f32x4& v = acc[nh][q >> 2][g][q & 3];
+                    float y[4] = {v[0], v[1], v[2], v[3]};
                     add_bias(y, bias[nh][g]);
                     if constexpr (EPI == EPI_BF16_GELU) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = gelu_tanh_f(y[j]);
                     }
-                    const int rl = (q >> 1) * 128 + wr * 64 + (q & 1) * 32 + fr, c = nh * 16 + wc * 4 + g;
-                    *reinterpret_cast<uint2*>(smem + rl * 512 + ((c ^ (rl & 15)) << 4) + fh * 8) =
+                    const int rl = (q >> 2) * 128 + wr * 64 + (q & 3) * 16 + fr, c = nh * 16 + wc * 4 + g * 2 + (quarter >> 1);
+                    *reinterpret_cast<uint2*>(smem + rl * 512 + ((c ^ fr) << 4) + (quarter & 1) * 8) =
                         make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
                 }
         __syncthreads();
@@ -715,15 +773,15 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
         }
     } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const long m = row0 + (q >> 1) * 128 + wr * 64 + (q & 1) * 32 + fr;
+        for (int q = 0; q < 8; ++q) {
+            const long m = row0 + (q >> 2) * 128 + wr * 64 + (q & 3) * 16 + fr;
 #pragma unroll
             for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int n = col0 + nh * 128 + wc * 32 + 8 * g + 4 * fh;
-                    const f32x16& a16 = acc[nh][q];
-                    float y[4] = {a16[4 * g], a16[4 * g + 1], a16[4 * g + 2], a16[4 * g + 3]};
+                for (int g = 0; g < 2; ++g) {
+                    const int n = col0 + nh * 128 + wc * 32 + 16 * g + 4 * quarter;
+                    const f32x4& v = acc[nh][q >> 2][g][q & 3];
+                    float y[4] = {v[0], v[1], v[2], v[3]};
                     add_bias(y, bias[nh][g]);
                     if (m < A.rows && n < W.rows) store4<EPI>(o, m, n, y);
                 }

@@ -51,8 +51,8 @@ def test_mxfp4_big_kernel_loop(mx):
     found = kernels(mx, "gemm_mxfp4_big_kernel")
     assert len(found) == 5                                         # one per epilogue
     for name, body in found.items():
-        loop = next(b for b in blocks(body) if count(b, "v_mfma") == 32 and count(b, "global_load_lds") == 10)
-        assert count(loop, "v_mfma_scale_f32_32x32x64_f8f6f4") == 32
+        loop = next(b for b in blocks(body) if count(b, "v_mfma") == 64 and count(b, "global_load_lds") == 10)
+        assert count(loop, "v_mfma_scale_f32_16x16x128_f8f6f4") == 64
         assert count(loop, "s_barrier") == 8
         waits = [i for i in loop if i.startswith("s_waitcnt") and "vmcnt" in i]
         assert len(waits) == 3 and all("vmcnt(10)" in w for w in waits), waits
