@@ -23,10 +23,12 @@
 // a document is never read, and a masked score is -inf whatever it was.
 //
 // What bounds it.  D = 128, long documents: the matrix pipe and the chip's power (20280, 1560, 14040 and 3600 tokens, 40
-// heads: 10.8 ms = 1180 TFLOP/s; one document of 20280 as fast as attn.hip).  D = 64: vector instructions (197 a tile and
+// heads: 10.8 ms = 1180 TFLOP/s; one document of 20280 as fast as attn.hip).  16x16x32 instructions instead of 32x32x16 would
+// take 12 % less power a product, but twice as many of them and the two queries that a lane then serves cost issue slots: 3 %
+// slower (one document), 5 to 20 % (short ones).  D = 64: vector instructions (197 a tile and
 // wave beside 16 matrix ones: 970 TFLOP/s), the more so with a cap (two transcendental instructions a score: 500).  Few
-// tokens: bytes of K and V (8 tokens against 80150 keys, 8 key heads: 76 us with the join = 4.4 TB/s).  Prompts of
-// some hundred tokens: the start and the last, partly filled round (8 of them, 16 heads of 64, a prefix: 47 us, 62 capped).
+// tokens: bytes of K and V (8 tokens against 80150 keys, 8 key heads: 72 us with the join = 4.6 TB/s).  Prompts of
+// some hundred tokens: the start and the last, partly filled round (8 of them, 16 heads of 64, a prefix: 45 us, 60 capped).
 #include "common.h"
 
 namespace {
@@ -161,6 +163,15 @@ __device__ __forceinline__ float* ws_stat(const Args& a, int part, long row) {
     return a.ws + a.max_splits * rows * D + (part * rows + row) * 2;
 }
 
+// 16 bytes a lane from `base + off` to 1 KiB of LDS.  As assembly because the compiler would wait for every DMA in flight ahead
+// of the next transposed read of LDS, whatever either touches: half a step after their start (documents of 700 and 300 queries
+// against 700 and 9000 keys 100 us against 70; 20280 and 14040 against 131 and 550 keys 109 against 101; one long document 0 to 1 %).
+// The waits stand at the ends of the steps, before the barrier that precedes the reads.
+__device__ __forceinline__ void dma_1k(const char* base, unsigned off, char* dst) {
+    const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>((lds_ptr)dst));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "m0", "memory");
+}
+
 // DMA of one operand: 64-row tiles HBM -> LDS.  A wave's instruction covers RPI rows; rows past the document's last key
 // repeat it.  Tile bases advance in 64 bits, offsets inside a tile are 32 bits.
 template <int D, int NW, bool IS_K>
@@ -190,11 +201,11 @@ struct Stream {
         if (NW > 1 && lim >= BKV - 1) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                __builtin_amdgcn_global_load_lds(tb + off[NW > 1 ? i : 0], (lds_ptr)(dst + (i * NW + wave) * 1024), 16, 0, 0);
+                dma_1k(tb, off[NW > 1 ? i : 0], dst + (i * NW + wave) * 1024);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                __builtin_amdgcn_global_load_lds(tb + offset(i, lim, wave, lane), (lds_ptr)(dst + (i * NW + wave) * 1024), 16, 0, 0);
+                dma_1k(tb, offset(i, lim, wave, lane), dst + (i * NW + wave) * 1024);
         }
     }
 };
@@ -340,8 +351,7 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
 // RAW (capped form): tile t's scores are not capped yet.  The cap is monotonic, so the running maximum needs it for one
 // value of a row, and the rest pass through it between this step's products, on their way into the exponential (packed
 // prompts with a cap 62 us; as a pass of its own between the two products 66 us).  Masked scores must not pass through it:
-// such tiles are capped first, then masked.  Three buffers of K and V instead of two: D = 64 10 % slower (the
-// buffers' addresses cost vector instructions; the loads are in time).
+// such tiles are capped first, then masked.
 template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT, bool RAW>
 __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
                                           const f32x16& c0, const f32x16& c1, f32x16& n0, f32x16& n1, float& mx, bool& need,
@@ -502,6 +512,9 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
         vst.stage(t0, smem + 2 * TILE, wave, lane);
         if (t0 + 1 < t1) kst.stage(t0 + 1, smem + TILE, wave, lane);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // Q has landed, too: said here, or the compiler waits for it (and every DMA with it) in the loop
+#pragma unroll
+        for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qf[i]));
         __syncthreads();
         f32x16 a0, a1, b0, b1;
         float mx = -3.0e38f;

@@ -73,3 +73,7 @@ def test_packed_attention_loop(tmp_path):
                  and count(b, "v_cndmask") < 8 and count(b, "ds_read_b64_tr_b16") >= mfma // 2]
         assert steps, f"no steady-state step found for head_dim {d}"
         assert all(count(b, "scratch_") == 0 for b in steps)
+        # the DMA of a step is waited for at its end, not ahead of the reads of V
+        for b in steps:
+            reads = [i for i, x in enumerate(b) if x.startswith("ds_read_b64_tr_b16")]
+            assert not [x for x in b[:reads[-1]] if x.startswith("s_waitcnt") and "vmcnt" in x]
