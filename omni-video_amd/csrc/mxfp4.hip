@@ -491,8 +491,8 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
 // that the chip then holds, and operands of zeros run 25 % faster.  The instruction shape is a matter of power, too: a loop
 // of products of Gaussian values alone holds 6.8 PFLOP/s as 32x32x64, 7.4 as 16x16x128 (fewer accumulators pass by per
 // product), 7.55 where only one operand changes from one to the next; the whole product gains 2 to 4 %.
-// 40560 x 8960 x 1536: 337 us bf16, 403 with GELU, 440 with the GELU quantised: with six k-groups a tile the epilogue is a
-// third of the time (its vector work and the stores).
+// 40560 x 8960 x 1536: 333 us bf16, 398 with GELU, 400 with the GELU quantised, 460 fp32: with six k-groups a tile the
+// epilogue is a third of the time (its vector work and the stores).
 // Not better: four waves of 128 x 128 outputs (4.3 PFLOP/s, a longer epilogue); 128 x 256 tiles in two workgroups per CU
 // (long K 3.8 PFLOP/s; short K with GELU 406 us against 421 then); the closing barriers ahead of a phase's last products
 // (2000 x 5120 x 5120 36.5 us against 34: the next reads wait behind them).
@@ -771,6 +771,52 @@ __device__ __forceinline__ void big_tile(const Operand& A, const Operand& W, con
                 }
             }
         }
+    } else if constexpr (!NARROW) {
+        // fp32 rows through LDS in two halves of 128 rows of 1 KiB (chunk c of row r at c ^ (r & 15)): a wave reads and writes
+        // whole rows of the tile (40560 x 8960 x 1536 with a residual 702 us, 64-byte pieces straight from the registers 826)
+        const int n = col0 + lane * 4;
+        const bool inside = n < W.rows;
+        const float4 gate = EPI == EPI_RESID && o.gate && inside ? *reinterpret_cast<const float4*>(o.gate + n) : make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+        for (int mh = 0; mh < 2; ++mh) {
+            if (mh) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const f32x4& v = acc[nh][mh][g][i];
+                        float y[4] = {v[0], v[1], v[2], v[3]};
+                        add_bias(y, bias[nh][g]);
+                        const int rl = wr * 64 + i * 16 + fr, c = nh * 32 + wc * 8 + g * 4 + quarter;
+                        *reinterpret_cast<f32x4*>(smem + rl * 1024 + ((c ^ fr) << 4)) = (f32x4){y[0], y[1], y[2], y[3]};
+                    }
+            __syncthreads();
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                f32x4 xs[8];
+                const long m0 = row0 + mh * 128 + b * 64 + wave;               // rows m0, m0 + 8, ...
+                float* ob = reinterpret_cast<float*>(o.out) + m0 * o.ldo + n;
+                if constexpr (EPI == EPI_RESID) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (m0 + 8 * i < A.rows && inside) xs[i] = *reinterpret_cast<const f32x4*>(ob + 8 * i * o.ldo);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int rl = b * 64 + 8 * i + wave;
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(smem + rl * 1024 + ((lane ^ (rl & 15)) << 4));
+                    if (m0 + 8 * i >= A.rows || !inside) continue;
+                    if constexpr (EPI == EPI_RESID)
+                        *reinterpret_cast<f32x4*>(ob + 8 * i * o.ldo) =
+                            (f32x4){fmaf(y[0], gate.x, xs[i][0]), fmaf(y[1], gate.y, xs[i][1]), fmaf(y[2], gate.z, xs[i][2]),
+                                    fmaf(y[3], gate.w, xs[i][3])};
+                    else
+                        *reinterpret_cast<f32x4*>(ob + 8 * i * o.ldo) = y;
+                }
+            }
+        }
     } else {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -799,6 +845,13 @@ __global__ void __launch_bounds__(512, 2) gemm_mxfp4_big_kernel(Operand A, Opera
     const int first = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
     const int count = q + (xcd < r ? 1 : 0);
     const int per_xcd = (gridDim.x + 7) >> 3;
+    // All tiles take equally long, so the workgroups of a launch store at the same time and then all compute.  Quarters of
+    // them start 3.7 us apart, the ones with a tile fewer last: 40560 x 4608 x 1536 191 us without, 171 with, with GELU 232 and
+    // 203, quantised 243 and 220; 4500 x 8960 x 1536 50 and 44.  With long K the stores are a small part and the delay is lost
+    // (40560 x 1536 x 8960: 254 without, 261 with), and below two rounds it can cost a round (3000 x 8960 x 1536 quantised:
+    // 39 without, 44 with)
+    if (groups <= 20 && nwg >= 2 * (int)gridDim.x)
+        for (int i = (int)(blockIdx.x >> 3) * 4 / per_xcd; i > 0; --i) __builtin_amdgcn_s_sleep(127);
     for (int t = blockIdx.x >> 3; t < count; t += per_xcd) {
         big_tile<EPI>(A, W, o, groups, tiles_m, tiles_n, GM, wide, first + t, big_smem);
         __syncthreads();          // the LDS buffers are staged again by the next tile
