@@ -688,11 +688,13 @@ def gemm_fp8(a8, w8, w_scale, out, bias=None, epilogue=EPI_BF16, a_scale=None, a
 
 def _call_on(index, name, *args):
     """_call on the current stream (appended as the last argument) of device `index`, made current for the call."""
-    if index == torch.cuda.current_device():
-        _call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    global CALLS
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            _call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            return _call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    CALLS += 1
+    if getattr(_lib or lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index)) != 0:
+        raise RuntimeError(f"{name}: {_lib.ovd_last_error().decode()}")
 
 
 def _one_device(*tensors):

@@ -85,7 +85,7 @@ class MXFP4Matrix:
     def dequantize(self, dtype=BF16, out=None):
         """The values it stands for, [rows, cols] bf16 or fp32 (exact in both)."""
         if out is None:
-            out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.buf.device)
+            out = self.buf.new_empty((self.rows, self.cols), dtype=dtype)
         return H.mxfp4_dequant(self, out)
 
 
@@ -98,8 +98,8 @@ def _no_grad(*tensors):
 def _rows2d(x):
     """x [..., K] as [M, K] with unit column stride and rows on 16-byte boundaries (a copy where it has none)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    ld = x2.stride(0)
-    if x2.stride(1) != 1 or ld < x2.shape[1] or (ld * x2.element_size()) % 16 or x2.data_ptr() % 16:
+    ld, step = x2.stride()
+    if step != 1 or ld < x2.shape[1] or (ld * x2.element_size()) % 16 or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 
@@ -157,7 +157,7 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
         if gate is not None:
             raise ValueError("mxfp4_linear: gate goes with residual")
         if out is None:
-            out = torch.empty((*lead, N), dtype=out_dtype, device=weight.buf.device)
+            out = weight.buf.new_empty((*lead, N), dtype=out_dtype)
         if gelu and out.dtype != BF16:
             raise TypeError("mxfp4_linear: gelu writes bf16")
         epi = H.EPI_BF16_GELU if gelu else (H.EPI_BF16 if out.dtype == BF16 else H.EPI_F32)
