@@ -123,7 +123,7 @@ def test_ocp_round_trip(X):
 
 SHAPES = [(1, 4, 32), (1, 5120, 5120), (2, 36, 288), (17, 260, 96), (31, 128, 1024), (32, 1536, 256), (33, 64, 2336),
           (64, 512, 320), (130, 100, 512), (550, 1536, 8960), (700, 772, 4096), (2049, 512, 1536), (1300, 1280, 96),
-          (8000, 1100, 512), (3333, 2564, 1056), (4127, 2052, 288), (700, 1252, 544)]
+          (8000, 1100, 512), (3333, 2564, 1056), (4127, 2052, 288), (700, 1252, 544), (20001, 2308, 288)]
 
 
 def close(got, want, bound, dtype):
@@ -165,7 +165,7 @@ def test_linear_epilogues(X, M, N, K):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 32, 64), (5, 96, 512), (33, 544, 288), (550, 1536, 1536), (300, 8960, 512),
-                                   (4127, 2080, 288), (8000, 1280, 512), (700, 1248, 544)])
+                                   (4127, 2080, 288), (8000, 1280, 512), (700, 1248, 544), (20001, 2336, 288)])
 def test_linear_with_quantised_output(X, M, N, K):
     """the output operand = the quantisation of the fp32 result: equal where the fp32 value is not within its own error
     of a border of the rounding or of a power of two of the block's largest magnitude"""
@@ -208,7 +208,7 @@ def test_linear_exact_on_small_integers(X):
     """whole numbers with scale 1 have exact sums: a wrong lane, block order, nibble order or scale byte shows as a
     wrong whole number.  Blocks get different scales, so each scale has to meet its own block."""
     for M, N, K in ((40, 68, 608), (1, 132, 1056), (300, 512, 256), (1030, 1536, 768), (5000, 1668, 1312),
-                    (16000, 516, 512)):
+                    (16000, 516, 512), (20001, 2308, 288)):
         g = torch.Generator().manual_seed(M)
         lut = torch.tensor([0.0, 1.0, 2.0, 3.0, 4.0, 6.0])
         a = lut[torch.randint(0, 6, (M, K), generator=g)] * (torch.randint(0, 2, (M, K), generator=g) * 2 - 1)
