@@ -218,6 +218,26 @@ def test_attention_causal_and_prefix(P, Lq, Lk, N, Nk, D):
         check(P.packed_attention(q, k, v, cu(Lq), cu(Lk), max(Lq), max(Lk), causal=True, prefix=pt, softcap=cap), want, bound)
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("causal,Lq,Lk,N,Nk", [
+    (False, [1300, 1500], [1300, 1500], 16, 16), (False, [1300, 300], [1900, 1100], 32, 16),
+    (True, [1100, 1100, 1100, 1100, 600], [1100, 1100, 1200, 1000, 600], 40, 40)])
+def test_attention_of_enough_rows_for_wide_workgroups(P, causal, Lq, Lk, N, Nk, D):
+    q, k, v = inputs(Lq, Lk, N, Nk, D, 31 + D)
+    prefix = [0, 300, 5, 0, 600] if causal else None
+    pt = torch.tensor(prefix, dtype=torch.int32, device="cuda") if causal else None
+    for cap in (0.0, 20.0):
+        want, bound = ref_attention(q, k, v, Lq, Lk, causal, prefix, cap, D ** -0.5)
+        check(P.packed_attention(q, k, v, cu(Lq), cu(Lk), max(Lq), max(Lk), causal=causal, prefix=pt, softcap=cap), want, bound)
+        if causal:                                       # a hidden infinity: seen by the last two queries of the first document
+            vv = v.clone()
+            vv[Lk[0] - 2, 3, 7] = math.inf
+            o = P.packed_attention(q, k, vv, cu(Lq), cu(Lk), max(Lq), max(Lk), causal=True, prefix=pt, softcap=cap)
+            assert (o[Lq[0] - 2:Lq[0], 3, 7] == math.inf).all()
+            o[Lq[0] - 2:Lq[0], 3, 7] = want[Lq[0] - 2:Lq[0], 3, 7].to(BF16)
+            check(o, want, bound)
+
+
 def test_attention_large_scores(P):
     """scores of several hundred, one dominating key late in the row, and capped ones"""
     Lq, Lk = [70, 3], [500, 400]
