@@ -130,6 +130,8 @@ def mxfp4_linear(x, weight, bias=None, gelu=False, out_dtype=BF16, out=None, res
     bias bf16 [N]; gelu: tanh-GELU (bf16 output).  Returns [..., N] in out_dtype (bf16 or fp32), written to `out` if given.
     residual: fp32 [..., N], updated in place as residual += y * gate[n] (gate fp32 [N] or None) and returned; out and
     residual may be x itself.
+    The sum over K is in a fixed order that depends on the sizes: the same row in a call of more rows may differ in its
+    last bit.
     quantize_output (with gelu, N a multiple of 32): the result as an MXFP4Matrix [M, N] (`out` if given), quantised from
     fp32 in the product's own pass: the input of the next layer."""
     if not isinstance(weight, MXFP4Matrix):
