@@ -355,7 +355,8 @@ int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos
  * h / (q_heads / kv_heads)).  Document d: query rows [cu_q[d], cu_q[d+1]), key rows [cu_k[d], cu_k[d+1]) (device int32
  * [docs + 1], ascending; values are clamped to the tensors).  Query i of a document with Lq queries and Lk keys sees
  * its first Lk keys, with `causal` its first max(i + Lk - Lq + 1, prefix[d]) (prefix: device int32 [docs] or NULL).
- * softcap > 0: scores s become softcap * tanh(s / softcap).  A query that sees no key gets zeros; rows outside every
+ * softcap > 0: scores s become softcap * tanh(s / softcap), off by at most 2^-20 of the cap up to 256 and 2^-18 of the
+ * score above.  A query that sees no key gets zeros; rows outside every
  * document are not written; keys and values outside a document do not enter it, whatever they hold.  out may be q
  * itself (same strides).
  * max_q / max_k: the longest document as the host knows it; they choose the launch (any value gives right results).

@@ -69,6 +69,7 @@ struct Args {
     int total_q, total_k, docs, kv_heads, group, causal;
     float scale_log2;                         // softmax scale * log2(e)
     float cap_in, cap_out;                    // 2 scale log2(e) / cap, cap log2(e)  (capped form)
+    float cap_x;                              // scale / cap
     int row_blocks, stripes;
     int chunk, max_splits;                    // split form: key tiles a work item should have, most parts of a document
     float* ws;                                // partial results of the parts
@@ -223,14 +224,26 @@ __device__ __forceinline__ bf16x8 read_v(const char* sv, int st, int db, int lan
     return __builtin_bit_cast(bf16x8, make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
 }
 
-// a capped score in units of log2, minus `minus`: cap log2(e) tanh(s scale / cap), tanh(x) = 1 - 2 / (1 + e^2x) (both ends
-// saturate without overflow)
+// a capped score in units of log2, minus `minus`: cap log2(e) tanh(x), x = s scale / cap, tanh(x) = 1 - 2 / (1 + e^2x) (both
+// ends saturate without overflow).  The difference cancels for small x: a score is off by up to 2^-21 of the cap, whatever
+// the score.  That is 1.2e-4 at SMALL_CAP, next to nothing beside the bf16 rounding of the probabilities; above it (LARGE)
+// scores below a quarter of the cap take the odd series instead, s (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315), cut off below
+// 2^-21 of the score, and what is left of the form above is below 2^-18 of the score.  As its own instantiations, because
+// the series costs what it does not bring to small caps (packed prompts 80 us against 62; causal, 20280 tokens, 12 heads 1759 against 1475).
+constexpr float SMALL_CAP = 256.f;
+
+template <bool LARGE>
 __device__ __forceinline__ float capped(float s, const Args& a, float minus) {
-    return __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.cap_in)), a.cap_out - minus);
+    const float far = __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * a.cap_in)), a.cap_out - minus);
+    if (!LARGE) return far;
+    const float x = s * a.cap_x, x2 = x * x;
+    const float p = __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+    return __builtin_fabsf(x) < 0.25f ? __builtin_fmaf(s * a.scale_log2, p, -minus) : far;
 }
+template <bool LARGE>
 __device__ __forceinline__ void cap_scores(f32x16& s, const Args& a) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[j] = capped(s[j], a, 0.f);
+    for (int j = 0; j < 16; ++j) s[j] = capped<LARGE>(s[j], a, 0.f);
 }
 
 __device__ __forceinline__ void mask_scores(f32x16& s0, f32x16& s1, int key0, int nvis, int hi) {
@@ -262,7 +275,7 @@ __device__ __forceinline__ bool tile_not_finite(const char* sv, int lane) {
     return __any(mx[0] >= 0x7f80 || mx[1] >= 0x7f80);
 }
 
-template <int D, int NW, bool CAP>
+template <int D, int NW, bool CAP, bool LARGE>
 __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
                                              char* smem, const Stream<D, NW, true>& kst, const Stream<D, NW, false>& vst, int t,
                                              int nvis, const Args& a, int wave, int lane) {
@@ -285,8 +298,8 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
         s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf1, qf[ks], s1, 0, 0, 0);
     }
     if (CAP) {
-        cap_scores(s0, a);
-        cap_scores(s1, a);
+        cap_scores<LARGE>(s0, a);
+        cap_scores<LARGE>(s1, a);
     }
     mask_scores(s0, s1, t * BKV, nvis, hi);
     const float sc = CAP ? 1.f : a.scale_log2;
@@ -352,7 +365,7 @@ __device__ __forceinline__ void careful_step(f32x16 (&o_acc)[D / 32], const bf16
 // value of a row, and the rest pass through it between this step's products, on their way into the exponential (packed
 // prompts with a cap 62 us; as a pass of its own between the two products 66 us).  Masked scores must not pass through it:
 // such tiles are capped first, then masked.
-template <int D, int NW, bool CAP, bool HAS_NEXT, bool MASK_NEXT, bool RAW>
+template <int D, int NW, bool CAP, bool LARGE, bool HAS_NEXT, bool MASK_NEXT, bool RAW>
 __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 (&qf)[D / 16], float& m_c, float& l_run,
                                           const f32x16& c0, const f32x16& c1, f32x16& n0, f32x16& n1, float& mx, bool& need,
                                           const char* sk_next, const char* sv_cur, const Stream<D, NW, true>& kst, char* k_dst,
@@ -378,7 +391,7 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
     const float sc = CAP ? 1.f : a.scale_log2;
     float rs0 = 0.f, rs1 = 0.f;
     uint32_t pw[16];
-#define EXPONENT(x) (RAW ? capped(x, a, m_c) : CAP ? (x) - m_c : __builtin_fmaf(x, sc, -m_c))
+#define EXPONENT(x) (RAW ? capped<LARGE>(x, a, m_c) : CAP ? (x) - m_c : __builtin_fmaf(x, sc, -m_c))
 #define SOFTMAX_PAIR(i)                                                                                    \
     do {                                                                                                   \
         const f32x16& c_ = (i) < 8 ? c0 : c1;                                                              \
@@ -420,8 +433,8 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
         __builtin_amdgcn_sched_barrier(0);
     }
     if (HAS_NEXT && MASK_NEXT && CAP) {
-        cap_scores(n0, a);
-        cap_scores(n1, a);
+        cap_scores<LARGE>(n0, a);
+        cap_scores<LARGE>(n1, a);
     }
     if (HAS_NEXT && MASK_NEXT) mask_scores(n0, n1, (t + 1) * BKV, nvis, hi);
     float nmx = -3.0e38f;
@@ -446,7 +459,7 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
             for (int r = 0; r < 16; r += 2) nmx = max3(nmx, n[r], n[r + 1]);
             asm volatile("" : "+v"(nmx));
             if (st == 3) {
-                mx = CAP ? (MASK_NEXT ? half_max(nmx) : capped(half_max(nmx), a, 0.f)) : half_max(nmx) * a.scale_log2;
+                mx = CAP ? (MASK_NEXT ? half_max(nmx) : capped<LARGE>(half_max(nmx), a, 0.f)) : half_max(nmx) * a.scale_log2;
                 need = __any(mx > m_c + RESCALE_THR);
             }
         }
@@ -458,7 +471,7 @@ __device__ __forceinline__ void pipe_step(f32x16 (&o_acc)[D / 32], const bf16x8 
 }
 
 // one work item: 32 NW rows of document `doc` under key head kvh, part `part` of `parts` of their keys
-template <int D, int NW, bool CAP, bool SPLIT>
+template <int D, int NW, bool CAP, bool LARGE, bool SPLIT>
 __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int doc, int rb, int part, int parts) {
     constexpr int ROWB = D * 2;                          // bytes per K / V row
     constexpr int TILE = BKV * ROWB;                     // bytes per tile; LDS: K[2] | V[2]
@@ -532,15 +545,15 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
             }
             if (t0 >= tf) {
                 if (CAP) {
-                    cap_scores(a0, a);
-                    cap_scores(a1, a);
+                    cap_scores<LARGE>(a0, a);
+                    cap_scores<LARGE>(a1, a);
                 }
                 mask_scores(a0, a1, t0 * BKV, nvis, hi);
             }
             float nmx = -3.0e38f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) nmx = max3(nmx, a0[r], a1[r]);
-            mx = CAP ? (t0 < tf ? capped(half_max(nmx), a, 0.f) : half_max(nmx)) : half_max(nmx) * a.scale_log2;
+            mx = CAP ? (t0 < tf ? capped<LARGE>(half_max(nmx), a, 0.f) : half_max(nmx)) : half_max(nmx) * a.scale_log2;
             need = __any(mx > m_c + RESCALE_THR);
         }
         __syncthreads();      // every wave is done with K(t0) before K(t0 + 2) overwrites it
@@ -548,7 +561,7 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
 #define PIPE_STEP(HAS_NEXT, MASK_NEXT, C0, C1, N0, N1, U)                                                           \
     do {                                                                                                            \
         const int u_ = (U), t_ = t0 + u_;                                                                           \
-        pipe_step<D, NW, CAP, HAS_NEXT, MASK_NEXT, CAP && HAS_NEXT && !MASK_NEXT>(                                  \
+        pipe_step<D, NW, CAP, LARGE, HAS_NEXT, MASK_NEXT, CAP && HAS_NEXT && !MASK_NEXT>(                                  \
             o_acc, qf, m_c, l_run, C0, C1, N0, N1, mx, need,                                                        \
                                                    smem + ((u_ + 1) & 1) * TILE, smem + (2 + (u_ & 1)) * TILE, kst, \
                                                    smem + (u_ & 1) * TILE, t_ + 2 < t1, vst,                        \
@@ -569,8 +582,8 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
             ++u;
         }
         if (CAP && t0 < tf) {                 // the last whole tile
-            cap_scores(a0, a);
-            cap_scores(a1, a);
+            cap_scores<LARGE>(a0, a);
+            cap_scores<LARGE>(a1, a);
         }
         for (; t0 + u + 1 < tw; ++u) {
             PIPE_STEP(true, true, a0, a1, b0, b1, u);
@@ -607,7 +620,7 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o_acc[i][j] = 0.f;
             for (int t = t0; t < t1; ++t)
-                careful_step<D, NW, CAP>(o_acc, qf, m_c, l_run, smem, kst, vst, t, nvis, a, wave, lane);
+                careful_step<D, NW, CAP, LARGE>(o_acc, qf, m_c, l_run, smem, kst, vst, t, nvis, a, wave, lane);
         }
     }
     l_run = half_sum(l_run);
@@ -654,7 +667,7 @@ __device__ __forceinline__ void attend(const Args& a, char* smem, int kvh, int d
 // unit b % stripes, and an XCD takes kv_heads * stripes / 8 consecutive units: a head's K / V stream is fetched into as
 // few L2s as possible, and XCDs that share a head get the same mix of documents and (causal) lengths (contiguous ranges
 // instead of stripes: 1040 against 1150 TFLOP/s with 12 heads over documents of 20280, 1560, 14040 and 3600 tokens).
-template <int D, int NW, bool CAP>
+template <int D, int NW, bool CAP, bool LARGE>
 __global__ void __launch_bounds__(64 * NW, 2) attn_packed_kernel(Args a) {
 #ifdef __HIP_DEVICE_COMPILE__     // the host pass has no use for the body (and refuses register constraints in shared parts of it)
     extern __shared__ __attribute__((aligned(16))) char smem[];   // (K | V)[2]
@@ -667,14 +680,14 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_packed_kernel(Args a) {
     if (!find_block<32 * NW, false>(a, blk, threadIdx.x & 63, doc, rb, part, parts)) return;
     doc = __builtin_amdgcn_readfirstlane(doc);
     rb = __builtin_amdgcn_readfirstlane(rb);
-    attend<D, NW, CAP, false>(a, smem, kvh, doc, rb, 0, 1);
+    attend<D, NW, CAP, LARGE, false>(a, smem, kvh, doc, rb, 0, 1);
 #endif
 }
 
 // Few query rows: the keys of a document are split into parts of about `chunk` tiles, all of one size per document, so
 // that documents of very different lengths fill the chip evenly.  Workgroups go on with further items a grid away: the
 // host sizes the grid by the lengths that it was told.  A document in one part is finished here, the others by the join.
-template <int D, int NW, bool CAP>
+template <int D, int NW, bool CAP, bool LARGE>
 __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_split_kernel(Args a) {
 #ifdef __HIP_DEVICE_COMPILE__
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -686,7 +699,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) attn_packed_split_ke
         rb = __builtin_amdgcn_readfirstlane(rb);
         part = __builtin_amdgcn_readfirstlane(part);
         parts = __builtin_amdgcn_readfirstlane(parts);
-        attend<D, NW, CAP, true>(a, smem, kvh, doc, rb, part, parts);
+        attend<D, NW, CAP, LARGE, true>(a, smem, kvh, doc, rb, part, parts);
         __syncthreads();                      // the output staging of this item before the tiles of the next
     }
 #endif
@@ -856,6 +869,7 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.cap_in = softcap > 0.f ? 2.f * a.scale_log2 / softcap : 0.f;
     a.cap_out = softcap * 1.4426950408889634f;
+    a.cap_x = softcap > 0.f ? softmax_scale / softcap : 0.f;
     const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, D, max_q, max_k, causal);
     // no (or too small a) workspace: every document in one part
     const long part_bytes = total_q * q_heads * (D + 2) * (long)sizeof(float);
@@ -879,20 +893,24 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
             OVD_FAIL("attn_packed: cannot reserve %zu bytes of LDS", lds);                                      \
         hipLaunchKernelGGL((KERNEL), dim3((unsigned)grid), dim3(64 * NW), lds, st, a);                          \
     }
-#define PACKED_KIND(DD, CAP)                                                                                    \
+#define PACKED_KIND(DD, CAP, LARGE)                                                                             \
     {                                                                                                           \
-        if (p.waves == 8) PACKED(PK(attn_packed_kernel, DD, 8, CAP), 8)                                         \
-        else if (!p.split) PACKED(PK(attn_packed_kernel, DD, 4, CAP), 4)                                        \
-        else if (p.waves == 4) PACKED(PK(attn_packed_split_kernel, DD, 4, CAP), 4)                              \
-        else PACKED(PK(attn_packed_split_kernel, DD, 1, CAP), 1)                                                \
+        if (p.waves == 8) PACKED(PK(attn_packed_kernel, DD, 8, CAP, LARGE), 8)                                  \
+        else if (!p.split) PACKED(PK(attn_packed_kernel, DD, 4, CAP, LARGE), 4)                                 \
+        else if (p.waves == 4) PACKED(PK(attn_packed_split_kernel, DD, 4, CAP, LARGE), 4)                       \
+        else PACKED(PK(attn_packed_split_kernel, DD, 1, CAP, LARGE), 1)                                         \
     }
-#define PK(K, DD, NW, CAP) (K<DD, NW, CAP>)
-    if (D == 128) {
-        if (softcap > 0.f) PACKED_KIND(128, true) else PACKED_KIND(128, false)
-    } else {
-        if (softcap > 0.f) PACKED_KIND(64, true) else PACKED_KIND(64, false)
+#define PACKED_CAP(DD)                                                                                          \
+    {                                                                                                           \
+        if (softcap > SMALL_CAP) PACKED_KIND(DD, true, true)                                                    \
+        else if (softcap > 0.f) PACKED_KIND(DD, true, false)                                                    \
+        else PACKED_KIND(DD, false, false)                                                                      \
     }
+#define PK(K, DD, NW, CAP, LARGE) (K<DD, NW, CAP, LARGE>)
+    if (D == 128) PACKED_CAP(128)
+    else PACKED_CAP(64)
 #undef PK
+#undef PACKED_CAP
 #undef PACKED_KIND
 #undef PACKED
     OVD_CHECK_LAUNCH("attn_packed");
