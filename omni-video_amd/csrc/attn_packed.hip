@@ -867,7 +867,8 @@ int ovd_impl_attn_packed(const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16
     a.total_q = (int)total_q; a.total_k = (int)total_k; a.docs = docs;
     a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.causal = causal;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
-    a.cap_in = softcap > 0.f ? 2.f * a.scale_log2 / softcap : 0.f;
+    // finite, however small the cap: a score of zero has to stay one
+    a.cap_in = softcap > 0.f ? fminf(2.f * a.scale_log2 / softcap, 3.0e38f) : 0.f;
     a.cap_out = softcap * 1.4426950408889634f;
     a.cap_x = softcap > 0.f ? softmax_scale / softcap : 0.f;
     const Plan p = plan_of(total_q, total_k, docs, kv_heads, a.group, D, max_q, max_k, causal);

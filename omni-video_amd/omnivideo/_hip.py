@@ -881,13 +881,16 @@ def attn_packed(q, k, v, cu_q, cu_k, out, max_q, max_k, causal=False, prefix=Non
         if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or docs < 1 or not t.is_contiguous():
             raise ValueError("attention: cu_q and cu_k must be int32 [documents + 1], prefix int32 [documents]")
     scale = float(softmax_scale) if softmax_scale is not None else D ** -0.5
+    softcap = float(softcap)
+    if 0.0 < softcap < 1e-30:       # scores of zero either way; as a 32-bit float it might become 0, which is no cap
+        softcap = 1e-30
     dev = _one_device(q, k, v, out, cu_q, cu_k, prefix, workspace)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("attention: workspace must be a contiguous device tensor")
     if Tq:
         _call_on(dev, "ovd_attn_packed_fwd_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), Tq, Tk,
                  cu_q.data_ptr(), cu_k.data_ptr(), docs, int(max_q), int(max_k), Nq, Nk, D, q_ld, k_ld, v_ld, o_ld,
-                 int(causal), None if prefix is None else prefix.data_ptr(), scale, float(softcap),
+                 int(causal), None if prefix is None else prefix.data_ptr(), scale, softcap,
                  None if workspace is None else workspace.data_ptr(),
                  0 if workspace is None else workspace.numel() * workspace.element_size())
     return out

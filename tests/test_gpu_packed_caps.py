@@ -91,3 +91,17 @@ def test_infinities_under_the_mask_with_a_large_cap(P, D):                      
         assert (o[298:300, 2:, 5].float() == value).all() and torch.isnan(o[429]).all()
         o[298:300, 2:, 5], o[429] = want[298:300, 2:, 5].to(o.dtype), want[429].to(o.dtype)
         check(o, want, bound)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("cap,scale", [(1e-20, None), (1e-37, 10.0), (1e-42, None), (1e-50, None), (1e-30, 1e20)])
+def test_caps_that_make_every_score_zero(P, cap, scale, D):                           # noqa: F811
+    """a cap of next to nothing leaves the mean of the values, for scores of zero, too"""
+    Lq, Lk = [70, 3], [500, 400]
+    q, k, v = inputs(Lq, Lk, 2, 2, D, 23)
+    q[5], k[600] = 0, 0
+    o = P.packed_attention(q, k, v, cu(Lq), cu(Lk), softcap=cap, softmax_scale=scale)
+    for a, b, c, d in ((0, 70, 0, 500), (70, 73, 500, 900)):
+        vd = v[c:d].double()
+        want, size = vd.mean(0).expand(b - a, -1, -1), vd.abs().mean(0).expand(b - a, -1, -1)
+        check(o[a:b], want, size * (2.0 ** -8 + (d - c + 64) * 2.0 ** -23))
