@@ -320,7 +320,10 @@ int ovd_flash_attn_qk8_fwd_bf16(const int8_t* q8, const float* q_scale, const in
  *   1: bf16 out of tanh-GELU, 2: fp32 out, 3: fp32 in-place out += y * gate[n] (gate NULL = 1), 4
  *   (OVD_EPI_MXFP4_GELU): tanh-GELU quantised from fp32 into an MXFP4 matrix [M, N] for a following product (out =
  *   its data, gate = its scale buffer, N % 32 == 0, ldo unused; ovd_gemm_mxfp4 only).  One rounding, of the
- *   stored value.  N % 4 == 0, K % 32 == 0, ldo % 4 == 0; bias bf16 [N] or NULL.  Sums are in a fixed order.
+ *   stored value.  N % 4 == 0, K % 32 == 0, ldo % 4 == 0; bias bf16 [N] or NULL.  Sums are in a fixed order, one of two that
+ *   M, N and K choose.
+ * ovd_gemm_mxfp4_as_rows: the same with the order that a call of order_rows rows has (0: M): rows that are computed in
+ *   parts, or with others beside them, get the same bits.
  * ovd_linear_mxfp4: ovd_mxfp4_quant of x [M, K] and ovd_gemm_mxfp4 in one call, a single launch for up to 8 rows;
  *   workspace: ovd_linear_mxfp4_workspace_bytes(M, K) (HOST) bytes, 16-byte aligned (0: none, may be NULL), free again
  *   when the call's work has finished.  out may share memory with x (x += f(x)); with few rows the call then needs
@@ -332,6 +335,9 @@ int ovd_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out, int 
                       void* stream);
 int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
                    void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream);
+int ovd_gemm_mxfp4_as_rows(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale,
+                           const uint16_t* bias, void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue,
+                           int order_rows, void* stream);
 #define OVD_EPI_MXFP4_GELU 4
 int64_t ovd_linear_mxfp4_workspace_bytes(int M, int K);
 int ovd_linear_mxfp4(const void* x, int x_is_f32, int64_t ldx, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,

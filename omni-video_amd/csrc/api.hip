@@ -45,7 +45,7 @@ long ovd_impl_mxfp4_scale_bytes(long, long);
 int ovd_impl_mxfp4_quant(const void*, int, long, uint8_t*, uint8_t*, int, int, hipStream_t);
 int ovd_impl_mxfp4_dequant(const uint8_t*, const uint8_t*, void*, int, long, int, int, hipStream_t);
 int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
-                        const float*, int, int, int, int, hipStream_t);
+                        const float*, int, int, int, int, int, hipStream_t);
 long ovd_impl_linear_mxfp4_workspace(int, int);
 int ovd_impl_linear_mxfp4(const void*, int, long, const uint8_t*, const uint8_t*, const bf16_t*, void*, long, const float*,
                           void*, long, int, int, int, int, hipStream_t);
@@ -355,7 +355,14 @@ int ovd_mxfp4_dequant(const uint8_t* data, const uint8_t* scale, void* out, int 
 int ovd_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale, const uint16_t* bias,
                    void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue, void* stream) {
     NONNULL(A); NONNULL(a_scale); NONNULL(W); NONNULL(w_scale); NONNULL(out);
-    return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, ST(stream));
+    return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, M, ST(stream));
+}
+
+int ovd_gemm_mxfp4_as_rows(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale,
+                           const uint16_t* bias, void* out, int64_t ldo, const float* gate, int M, int N, int K, int epilogue,
+                           int order_rows, void* stream) {
+    NONNULL(A); NONNULL(a_scale); NONNULL(W); NONNULL(w_scale); NONNULL(out);
+    return ovd_impl_gemm_mxfp4(A, a_scale, W, w_scale, bias, out, ldo, gate, M, N, K, epilogue, order_rows, ST(stream));
 }
 
 int64_t ovd_linear_mxfp4_workspace_bytes(int M, int K) { return M <= 0 || K <= 0 ? 0 : ovd_impl_linear_mxfp4_workspace(M, K); }

@@ -917,7 +917,7 @@ long ovd_impl_linear_mxfp4_workspace(int M, int K) {
 }
 
 int ovd_impl_gemm_mxfp4(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, const bf16_t*, void*, long,
-                        const float*, int, int, int, int, hipStream_t);
+                        const float*, int, int, int, int, int, hipStream_t);
 
 // the output side of both products
 static int check_out(int M, int N, int K, int epilogue, const void* out, long ldo, const void* bias, const void* gate,
@@ -954,7 +954,7 @@ int ovd_impl_linear_mxfp4(const void* x, int x_is_f32, long ldx, const uint8_t* 
                     need, workspace_bytes);
         uint8_t* data = (uint8_t*)workspace;
         if (ovd_impl_mxfp4_quant(x, x_is_f32, ldx, data, data + nd, M, K, st)) return 1;
-        return ovd_impl_gemm_mxfp4(data, data + nd, w_data, w_scale, bias, out, ldo, gate, M, N, K, epilogue, st);
+        return ovd_impl_gemm_mxfp4(data, data + nd, w_data, w_scale, bias, out, ldo, gate, M, N, K, epilogue, M, st);
     }
     OVD_REQUIRE(ldx >= K && ldx % (x_is_f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0,
                 "linear_mxfp4: rows must keep 16-byte alignment (ldx=%ld)", ldx);
@@ -980,8 +980,9 @@ int ovd_impl_linear_mxfp4(const void* x, int x_is_f32, long ldx, const uint8_t* 
 
 int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uint8_t* w_data, const uint8_t* w_scale,
                         const bf16_t* bias, void* out, long ldo, const float* gate, int M, int N, int K, int epilogue,
-                        hipStream_t st) {
+                        int order_rows, hipStream_t st) {
     if (check_out(M, N, K, epilogue, out, ldo, bias, gate, w_data, w_scale)) return 1;
+    OVD_REQUIRE(order_rows >= 0, "gemm_mxfp4: order_rows=%d is negative", order_rows);
     OVD_REQUIRE(reinterpret_cast<uintptr_t>(a_data) % 16 == 0 && reinterpret_cast<uintptr_t>(a_scale) % 4 == 0,
                 "gemm_mxfp4: operands must be 16-byte aligned");
     OVD_REQUIRE(epilogue != EPI_MX_GELU || (out != a_data && out != w_data), "gemm_mxfp4: the output matrix is one of the operands");
@@ -1017,12 +1018,15 @@ int ovd_impl_gemm_mxfp4(const uint8_t* a_data, const uint8_t* a_scale, const uin
     // 12 us against 47; 800 x 8960 x 1536: 31 against 15).  32 x 32 tiles, of which several share a CU, take 0.3 rounds of
     // 64 x 64 ones per tile and CU, and one such time to begin (64 x 1536 x 8960: 5.1 us against 10.2; 550: 15 against 12).
     const int outs = epilogue == EPI_MX_GELU ? ceil_div(N, KG) * KG : N;
-    const long tiny = (long)ceil_div(M, 32) * ceil_div(outs, 32), small = (long)ceil_div(M, 64) * ceil_div(outs, 64);
-    const long t_big = ceil_div((long)tiles_m * tiles_n, cus) * (23L + 6 * groups);
-    const long t_small = ceil_div(small, cus) * (16L + groups), t_tiny = 3 * (tiny + cus) * (16L + groups) / (10L * cus);
-    const bool big = groups >= 2 && t_big < min(t_small, t_tiny);
+    const auto t_small = [&](int rows) { return ceil_div((long)ceil_div(rows, 64) * ceil_div(outs, 64), cus) * (16L + groups); };
+    const auto t_tiny = [&](int rows) { return 3 * ((long)ceil_div(rows, 32) * ceil_div(outs, 32) + cus) * (16L + groups) / (10L * cus); };
+    // The 256 x 256 tiles add a row's products in another order than the other two, which share theirs: which of the two
+    // orders goes by order_rows, so that a caller whose rows come in parts of any size gets the same bits for each
+    const int as = order_rows > 0 ? order_rows : M;
+    const long t_big = ceil_div((long)ceil_div(as, TM) * tiles_n, cus) * (23L + 6 * groups);
+    const bool big = groups >= 2 && t_big < min(t_small(as), t_tiny(as));
     const int wide = (ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) ? 1 : 0;
-#define GEMM_CASE(E) case E: if (big) BIG(E) else if (t_tiny < t_small) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
+#define GEMM_CASE(E) case E: if (big) BIG(E) else if (t_tiny(M) < t_small(M)) DIRECT(1, 1, E) else DIRECT(2, 2, E) break;
     switch (epilogue) { GEMM_CASE(EPI_BF16) GEMM_CASE(EPI_BF16_GELU) GEMM_CASE(EPI_F32) GEMM_CASE(EPI_RESID) GEMM_CASE(EPI_MX_GELU) }
 #undef GEMM_CASE
 #undef BIG

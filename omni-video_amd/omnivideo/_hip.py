@@ -52,6 +52,7 @@ SIGNATURES = {
     "ovd_mxfp4_quant": [_p, _i, _l, _p, _p, _i, _i, _p],
     "ovd_mxfp4_dequant": [_p, _p, _p, _i, _l, _i, _i, _p],
     "ovd_gemm_mxfp4": [_p, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _p],
+    "ovd_gemm_mxfp4_as_rows": [_p, _p, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _i, _p],
     "ovd_linear_mxfp4_workspace_bytes": [_i, _i],
     "ovd_linear_mxfp4": [_p, _i, _l, _p, _p, _p, _p, _l, _p, _p, _l, _i, _i, _i, _i, _p],
     "ovd_rope_positions": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _l, _l, _i, _i, _i, _i, _p],
@@ -767,8 +768,9 @@ def _mx_out(name, out, M, N, bias, epilogue, gate):
     return _row_stride(name, out, N)
 
 
-def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
-    """out = epilogue(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; out [..., N] with a uniform row stride."""
+def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None, order_rows=0):
+    """out = epilogue(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; out [..., N] with a uniform row stride.
+    order_rows: sums in the order that a product of so many rows has (0: M)."""
     M, N, K = a.rows, w.rows, a.cols
     if w.cols != K:
         raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}]")
@@ -776,16 +778,17 @@ def gemm_mxfp4(a, w, out, bias=None, epilogue=EPI_BF16, gate=None):
     dev = _one_device(a.buf, w.buf, out, bias, gate)
     (ad, asc), (wd, wsc) = a.pointers(), w.pointers()
     if M:
-        _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), out.data_ptr(),
-                 ldo, None if gate is None else gate.data_ptr(), M, N, K, epilogue)
+        _call_on(dev, "ovd_gemm_mxfp4_as_rows", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                 ldo, None if gate is None else gate.data_ptr(), M, N, K, epilogue, order_rows)
     return out
 
 
 EPI_MXFP4_GELU = 4
 
 
-def gemm_mxfp4_gelu(a, w, out, bias=None):
-    """out (MXFP4 matrix [M, N]) = quantised gelu(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]."""
+def gemm_mxfp4_gelu(a, w, out, bias=None, order_rows=0):
+    """out (MXFP4 matrix [M, N]) = quantised gelu(a @ w.T + bias) on two MXFP4 matrices [M, K], [N, K]; order_rows as in
+    gemm_mxfp4."""
     M, N, K = a.rows, w.rows, a.cols
     if w.cols != K or out.rows != M or out.cols != N:
         raise ValueError(f"gemm_mxfp4: shape mismatch a[{M},{K}] w[{N},{w.cols}] out[{out.rows},{out.cols}]")
@@ -796,8 +799,8 @@ def gemm_mxfp4_gelu(a, w, out, bias=None):
     if M and od in (ad, wd):
         raise ValueError("gemm_mxfp4: the output matrix cannot be one of the operands")
     if M:
-        _call_on(dev, "ovd_gemm_mxfp4", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), od, N, osc, M, N, K,
-                 EPI_MXFP4_GELU)
+        _call_on(dev, "ovd_gemm_mxfp4_as_rows", ad, asc, wd, wsc, None if bias is None else bias.data_ptr(), od, N, osc, M, N, K,
+                 EPI_MXFP4_GELU, order_rows)
     return out
 
 

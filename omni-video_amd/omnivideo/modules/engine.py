@@ -203,7 +203,8 @@ class DiTEngine:
         channel, activations per token row inside the kernel that produces them (the GELU output
         with the fixed scale `ffn_act_scale`); "mxfp4": the same layers on MXFP4 operands (4-bit
         elements, one power-of-two scale per 32 values along the row; mxfp4.py), activations
-        quantised per call, the GELU output inside the product.
+        quantised per call, the GELU output inside the product, sums in the order that one unsharded branch's rows
+        call for (a row's bits do not depend on the batch or the ranks).
         attention: "bf16", or "int8": self-attention computes Q K^T on int8 operands (q with a scale per
         token and head, k per 64-key tile and head; softmax, P and P V unchanged); default: "int8"
         with precision "fp8" or "mxfp4", else "bf16".  Cross-attention, norms, the residual stream and the head
@@ -510,7 +511,7 @@ class DiTEngine:
         if self.precision == "fp8":
             H.gemm_fp8(self.h8, L["w8_" + name], L["s_" + name], out, L["b_" + name], H.EPI_BF16, a_scale=self.h_scale)
         elif self.precision == "mxfp4":
-            H.gemm_mxfp4(self.h4, L["w4_" + name], out, L["b_" + name], H.EPI_BF16)
+            H.gemm_mxfp4(self.h4, L["w4_" + name], out, L["b_" + name], H.EPI_BF16, order_rows=self.seq_len)
         else:
             H.gemm(self.h, L["w_" + name], out, L["b_" + name], H.EPI_BF16)
 
@@ -521,7 +522,8 @@ class DiTEngine:
             H.gemm_fp8(self.att8, L["w8_" + name], L["s_" + name], self.res, L["b_" + name], H.EPI_BF16,
                        a_scale=self.att_scale)
         elif self.precision == "mxfp4":
-            H.gemm_mxfp4(H.mxfp4_quant(att2, self.att4), L["w4_" + name], self.res, L["b_" + name], H.EPI_BF16)
+            H.gemm_mxfp4(H.mxfp4_quant(att2, self.att4), L["w4_" + name], self.res, L["b_" + name], H.EPI_BF16,
+                         order_rows=self.seq_len)
         else:
             H.gemm(att2, L["w_" + name], self.res, L["b_" + name], H.EPI_BF16)
 
@@ -594,8 +596,8 @@ class DiTEngine:
                 H.gemm_fp8(self.ffn8, L["w8_f2"], L["s_f2"], self.res, L["b_f2"], H.EPI_BF16,
                            a_scale_all=self.ffn_act_scale)
             elif self.precision == "mxfp4":
-                H.gemm_mxfp4_gelu(self.h4, L["w4_f0"], self.ffn4, L["b_f0"])
-                H.gemm_mxfp4(self.ffn4, L["w4_f2"], self.res, L["b_f2"], H.EPI_BF16)
+                H.gemm_mxfp4_gelu(self.h4, L["w4_f0"], self.ffn4, L["b_f0"], order_rows=self.seq_len)
+                H.gemm_mxfp4(self.ffn4, L["w4_f2"], self.res, L["b_f2"], H.EPI_BF16, order_rows=self.seq_len)
             else:
                 H.gemm(self.h, L["w_f0"], self.ffn, L["b_f0"], H.EPI_BF16_GELU)
                 H.gemm(self.ffn, L["w_f2"], self.res, L["b_f2"], H.EPI_BF16)

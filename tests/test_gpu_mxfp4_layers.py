@@ -34,14 +34,14 @@ def test_every_layer_is_its_own_product(monkeypatch):
         calls.append(("quant", x.data_ptr(), x.clone(), out, out.dequantize(F32)))
         return out
 
-    def on_gemm(a, w, out, bias=None, epilogue=H.EPI_BF16, gate=None):
+    def on_gemm(a, w, out, bias=None, epilogue=H.EPI_BF16, gate=None, **kw):
         assert epilogue == H.EPI_BF16 and gate is None
-        gemm(a, w, out, bias, epilogue)
+        gemm(a, w, out, bias, epilogue, **kw)
         calls.append(("gemm", a, a.dequantize(F32), w, bias, out.clone()))
         return out
 
-    def on_gelu(a, w, out, bias=None):
-        gelu(a, w, out, bias)
+    def on_gelu(a, w, out, bias=None, **kw):
+        gelu(a, w, out, bias, **kw)
         calls.append(("gelu", a, a.dequantize(F32), w, bias, out, out.dequantize(F32)))
         return out
 
@@ -95,3 +95,62 @@ def test_every_layer_is_its_own_product(monkeypatch):
 def test_sharded_forward_in_the_mode(heads, sp, seq_len):
     """equal bits: products of so few tiles add in one order, however many rows there are"""
     sharded_equals_unsharded(heads, sp, seq_len, "mxfp4")
+
+
+def forwards(precision, groups, comms=None):
+    """outputs of the forwards of a 3200-token model, one for each group of contexts (and communicator, as threads)"""
+    import threading
+    from omnivideo.modules.engine import DiTEngine
+    from omnivideo.utils import synthetic as syn
+    from test_gpu_sequence_parallel import build
+    cfg = syn.dit_config("tiny", dim=512, num_heads=4, ffn_dim=2560)
+    sd = syn.make_unified_state_dict(cfg, 0)
+    for i in range(cfg["num_layers"]):
+        # large terms that cancel, 8 k-groups apart: the small ones between them are rounded at the size of the large ones in
+        # one order of the sums and exact in the other
+        w0, b0, w2 = (sd[f"wan_model.blocks.{i}.ffn.{n}"] for n in ("0.weight", "0.bias", "2.weight"))
+        w0[2048:2080], b0[2048:2080] = w0[:32], b0[:32]
+        w2[:, :32] *= 2.0 ** 14
+        w2[:, 2048:2080] = -w2[:, :32]
+    wm = build(cfg, sd)
+    lat = syn.randn("in.lat", (16, 5, 32, 80), 1).cuda().to(BF16)
+    ts = torch.tensor([640.0], dtype=torch.float64, device="cuda")
+    text = [syn.randn("in.text", (10, cfg["text_dim"]), s).cuda().to(BF16) for s in (1, 2)]
+    outs, errs = [None] * len(groups), []
+
+    def run(i):
+        try:
+            eng = DiTEngine(wm, precision=precision)
+            eng.plan((5, 16, 40), 3200, len(groups[i]), comm=None if comms is None else comms[i])
+            eng.attn_ws = None                             # its split of the last query blocks goes by the launch's grid
+            out = torch.empty(len(groups[i]), 16, 5, 32, 80, device="cuda")
+            eng.forward(lat, ts, eng.encode_context([text[b] for b in groups[i]], wm.text_len), out)
+            torch.cuda.synchronize()
+            outs[i] = out
+        except Exception as e:          # noqa: BLE001
+            errs.append(e)
+            if comms is not None:
+                comms[i].sh.barrier.abort()
+
+    if comms is None:
+        for i in range(len(groups)):
+            run(i)
+    else:
+        th = [threading.Thread(target=run, args=(i,)) for i in range(len(groups))]
+        [t.start() for t in th]
+        [t.join(120) for t in th]
+    assert not errs, errs
+    return outs
+
+
+@pytest.mark.parametrize("precision", ["mxfp4", "fp8", "bf16"])
+def test_rows_do_not_depend_on_how_many_a_rank_or_a_batch_has(precision):
+    """one branch alone, two in a batch, and the batch over two or four ranks: equal bits, although other kernels compute
+    products of 6400 rows than of 3200 or 1600"""
+    from test_gpu_sequence_parallel import ThreadComm, _Shared
+    both, first, second = forwards(precision, ([0, 1], [0], [1]))
+    assert torch.equal(both, torch.cat((first, second)))
+    for n in (2, 4):
+        shared = _Shared(n)
+        for out in forwards(precision, [[0, 1]] * n, [ThreadComm(shared, r) for r in range(n)]):
+            assert torch.equal(out, both), f"{n} ranks: {int((out != both).sum())} of {both.numel()} differ"
