@@ -168,9 +168,11 @@ __device__ __forceinline__ float* ws_stat(const Args& a, int part, long row) {
 // of the next transposed read of LDS, whatever either touches: half a step after their start (documents of 700 and 300 queries
 // against 700 and 9000 keys 100 us against 70; 20280 and 14040 against 131 and 550 keys 109 against 101; one long document 0 to 1 %).
 // The waits stand at the ends of the steps, before the barrier that precedes the reads.
+// s_nop: m0 may be used one wait state after its write, an SGPR that a vector instruction wrote (the compiler spills to lanes
+// of vector registers and does not see the load in here) five.
 __device__ __forceinline__ void dma_1k(const char* base, unsigned off, char* dst) {
     const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>((lds_ptr)dst));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "m0", "memory");
 }
 
 // DMA of one operand: 64-row tiles HBM -> LDS.  A wave's instruction covers RPI rows; rows past the document's last key
