@@ -174,6 +174,13 @@ __device__ __forceinline__ void dma_1k(const char* base, unsigned off, char* dst
     const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>((lds_ptr)dst));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(off), "s"(base) : "m0", "memory");
 }
+// the same twice, STEP bytes of LDS apart, with one such wait
+template <int STEP>
+__device__ __forceinline__ void dma_2k(const char* base, unsigned off0, unsigned off1, char* dst) {
+    const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>((lds_ptr)dst));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_add_u32 m0, m0, %4\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %2, %3" ::"s"(m0), "v"(off0), "v"(off1), "s"(base), "n"(STEP) : "m0", "scc", "memory");
+}
 
 // DMA of one operand: 64-row tiles HBM -> LDS.  A wave's instruction covers RPI rows; rows past the document's last key
 // repeat it.  Tile bases advance in 64 bits, offsets inside a tile are 32 bits.
@@ -201,14 +208,17 @@ struct Stream {
     __device__ __forceinline__ void stage(int t, char* dst, int wave, int lane) const {
         const char* tb = base + (long)t * BKV * ld2;
         const int lim = lk - 1 - t * BKV;
-        if (NW > 1 && lim >= BKV - 1) {
+        const bool whole = NW > 1 && lim >= BKV - 1;
+        if constexpr (N == 1) {
+            dma_1k(tb, whole ? off[0] : offset(0, lim, wave, lane), dst + wave * 1024);
+        } else if (whole) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                dma_1k(tb, off[NW > 1 ? i : 0], dst + (i * NW + wave) * 1024);
+            for (int i = 0; i < N; i += 2)
+                dma_2k<NW * 1024>(tb, off[NW > 1 ? i : 0], off[NW > 1 ? i + 1 : 0], dst + (i * NW + wave) * 1024);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                dma_1k(tb, offset(i, lim, wave, lane), dst + (i * NW + wave) * 1024);
+            for (int i = 0; i < N; i += 2)
+                dma_2k<NW * 1024>(tb, offset(i, lim, wave, lane), offset(i + 1, lim, wave, lane), dst + (i * NW + wave) * 1024);
         }
     }
 };

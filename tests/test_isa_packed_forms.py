@@ -46,6 +46,8 @@ def test_dma_blocks_wait_for_their_scalar_operands(text):
         at = next(n for n, i in enumerate(block) if i.startswith("global_load_lds"))
         states = sum(1 + (int(i.split()[1]) if i.startswith("s_nop") else 0) for i in block[:at])
         assert states >= 5, block
+        for n, i in enumerate(block[1:], 1):                 # m0 is read one wait state after its write
+            assert not (i.startswith("global_load_lds") and re.search(r"\bm0,", block[n - 1])), block
         # m0 is this block's alone: written in front of the load, and used by nothing else in the file
         assert block[0].startswith("s_mov_b32 m0,")
     assert not [i for i in outside if re.search(r"\bm0\b", i)]
