@@ -350,7 +350,8 @@ int ovd_linear_mxfp4(const void* x, int x_is_f32, int64_t ldx, const uint8_t* W,
  * x_is_f32; dense heads, token strides ldx / ldo; out may be x), pos [tokens, n_axes] int32 (fp32 when pos_is_f32).
  * Pair p of a head turns by pos[t][axis[p]] * freq[p] REVOLUTIONS (freq double, axis int32, both [head_dim / 2] on the
  * device; axis outside [0, n_axes): the pair passes through).  interleaved: pairs (2p, 2p + 1), else (p, p + head_dim/2);
- * inverse: the opposite turn.  head_dim % 16 == 0, <= 512; n_axes <= 8.  Angles are 64-bit: positions may be large.
+ * inverse: the opposite turn.  head_dim % 16 == 0, <= 512; n_axes <= 8.  Angles are 64-bit: off by 2^-51 of the turns made at
+ * most (2e-7 turns for any int32 position); the rotation is fp32: 2^-20 of |x0| + |x1|, then the rounding to x's type.
  * The positions form of rope_apply (omnivideo/modules/model.py:37-65), which derives them from one grid per sample. */
 int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos, int pos_is_f32, int n_axes,
                        const double* freq, const int32_t* axis, void* out, int64_t ldo, int64_t tokens, int heads,
@@ -365,6 +366,7 @@ int ovd_rope_positions(const void* x, int x_is_f32, int64_t ldx, const void* pos
  * score above.  A query that sees no key gets zeros; rows outside every
  * document are not written; keys and values outside a document do not enter it, whatever they hold.  out may be q
  * itself (same strides).
+ * Softmax and sums are fp32; the probabilities are rounded to bf16 for their product with v.
  * max_q / max_k: the longest document as the host knows it; they choose the launch (any value gives right results).
  * workspace: with few query rows the keys are split over workgroups and joined, in
  * ovd_attn_packed_workspace_bytes(...) (HOST) bytes, 16-byte aligned; NULL or smaller: not split.  It holds no state

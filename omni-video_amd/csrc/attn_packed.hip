@@ -1,4 +1,6 @@
-// Attention over packed documents, forward: bf16 operands, fp32 softmax and accumulation.
+// Attention over packed documents, forward: bf16 operands, fp32 softmax and accumulation.  The probabilities are rounded to
+// bf16 for the second product (a matrix instruction takes both operands so; their sum is that of the unrounded ones): 2^-9 of
+// each, independently.  Outputs are 2.3e-3 off in relative L2, where fp32 probabilities and one rounding would leave 1.7e-3.
 //
 // Tokens of several documents (videos, images, prompts of different sizes) lie one after another in q [Tq, Nq, D] and
 // k, v [Tk, Nkv, D]; document d owns query rows [cu_q[d], cu_q[d+1]) and key rows [cu_k[d], cu_k[d+1]).  Query i of a
@@ -23,12 +25,14 @@
 // a document is never read, and a masked score is -inf whatever it was.
 //
 // What bounds it.  D = 128, long documents: the matrix pipe and the chip's power (20280, 1560, 14040 and 3600 tokens, 40
-// heads: 10.8 ms = 1180 TFLOP/s; one document of 20280 as fast as attn.hip).  16x16x32 instructions instead of 32x32x16 would
+// heads: 10.7 ms = 1190 TFLOP/s; one document of 20280 as fast as attn.hip).  16x16x32 instructions instead of 32x32x16 would
 // take 12 % less power a product, but twice as many of them and the two queries that a lane then serves cost issue slots: 3 %
 // slower (one document), 5 to 20 % (short ones).  D = 64: vector instructions (197 a tile and
-// wave beside 16 matrix ones: 970 TFLOP/s), the more so with a cap (two transcendental instructions a score: 500).  Few
-// tokens: bytes of K and V (8 tokens against 80150 keys, 8 key heads: 72 us with the join = 4.6 TB/s).  Prompts of
-// some hundred tokens: the start and the last, partly filled round (8 of them, 16 heads of 64, a prefix: 45 us, 60 capped).
+// wave beside 16 matrix ones: 970 TFLOP/s), the more so with a cap (two more transcendental instructions a score: 500).  Few
+// tokens: bytes of K and V (8 tokens against 80750 keys, 8 key heads: 73 us with the join = 4.5 TB/s).  Prompts of
+// some hundred tokens: the start and the last, partly filled round (8 of them, 16 heads of 64, a prefix: 44 us, 59 capped).
+// The four-wave form with split keys spills about 70 registers at D = 128 and reloads some of them in every step (700 and 300
+// queries against 700 and 9000 keys: 59 us before the join, 330 TFLOP/s); no other form spills.
 #include "common.h"
 
 namespace {

@@ -1,6 +1,6 @@
 // MXFP4 (OCP microscaling, E2M1 elements, one E8M0 scale per 32 values of a row): quantisation of row matrices and
-// the product of two of them, out = epilogue(A[M,K] * W[N,K]^T + bias[N]), on v_mfma_scale_f32_32x32x64_f8f6f4 with
-// fp4 operands.  A reduced-precision form of the linear layers beside the e4m3 one of fp8.hip (the reference runs
+// the product of two of them, out = epilogue(A[M,K] * W[N,K]^T + bias[N]), on fp4 operands of v_mfma_scale_f32_16x16x128_f8f6f4
+// (256 x 256 tiles) and v_mfma_scale_f32_32x32x64_f8f6f4 (fewer rows).  A reduced-precision form of the linear layers beside the e4m3 one of fp8.hip (the reference runs
 // these layers in bf16: omnivideo/modules/model.py:125-154, :159-179, :218-258).
 //
 // Definition of the quantisation (a block is 32 consecutive k of one row):
@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 // One workgroup = one row block x one k-group, a wave 8 of its rows.  A load instruction covers 8 rows x 64 k (8 lanes of
 // 8 values per row: whole 128-byte lines of bf16), a store instruction two runs of 8 rows x 16 bytes; the four lanes of an
 // MX block exchange their largest magnitude.  HBM-bound: 2 (4) bytes read and 17/32 written per value: 40560 x 8960 bf16
-// 165 us = 5.6 TB/s, back in 160 us (a wave over all 32 rows of the block: 186 and 180, and 550 x 8960 11.5 us instead of 4.3).
+// there and back 335 us = 5.5 TB/s (with a wave over all 32 rows of the block 366, and 550 x 8960 2.7 times as long).
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
 template <>
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(512) gemm_mxfp4_direct_kernel(Operand A, Opera
 
 // A handful of rows (M <= FEW_ROWS) straight from bf16 / fp32: every workgroup quantises all of x into LDS (a few thousand
 // values) under its first weight loads, so a token's layer is one launch.  A workgroup owns one block of 32 weight rows;
-// its waves take the k-groups in turn and meet as above.  Bound by the weights: one row of 5120 x 5120 5.4 us (launch
-// and one trip to memory 3, 13.9 MB of weights the rest); as two launches 8.  LDS: codes [group][ks][h][FEW_ROWS][16], scales
+// its waves take the k-groups in turn and meet as above.  Bound by the weights: one row of 5120 x 5120 5.6 us (launch
+// and one trip to memory 3, 13.9 MB of weights the rest, on the 160 CUs that have a block); as two launches 8.  LDS: codes [group][ks][h][FEW_ROWS][16], scales
 // [group][h][FEW_ROWS][4], then the partial sums.
 constexpr int FEW_ROWS = 8;
 constexpr int FEW_GRP = 8 * FEW_ROWS * 16 + 2 * FEW_ROWS * 4;       // LDS bytes per k-group
@@ -487,12 +487,12 @@ __global__ void __launch_bounds__(512) linear_mxfp4_few_kernel(const T* __restri
 // The tile layout makes every DMA instruction 1 KiB of consecutive memory and every fragment read four runs of 256 bytes of
 // LDS: no swizzle.  Scales travel the same way, one 256-byte instruction per row block and K-tile (8 KiB of LDS for two
 // buffers); they are issued with phase 4, so any four consecutive phases hold 10 DMA instructions of a wave.
-// 32760 x 5120 x 13824: 0.97 ms = 4.8 PFLOP/s, bound by power: the matrix pipe is busy 60 % of cycles at the 1.4 to 1.7 GHz
-// that the chip then holds, and operands of zeros run 25 % faster.  The instruction shape is a matter of power, too: a loop
+// 32760 x 5120 x 13824: 0.99 ms = 4.7 PFLOP/s, bound by power: the matrix pipe is busy 61 % of cycles at the 1.6 to 1.9 GHz
+// that the chip then holds, and operands of zeros take 785 us.  The instruction shape is a matter of power, too: a loop
 // of products of Gaussian values alone holds 6.8 PFLOP/s as 32x32x64, 7.4 as 16x16x128 (fewer accumulators pass by per
 // product), 7.55 where only one operand changes from one to the next; the whole product gains 2 to 4 %.
-// 40560 x 8960 x 1536: 333 us bf16, 398 with GELU, 400 with the GELU quantised, 460 fp32: with six k-groups a tile the
-// epilogue is a third of the time (its vector work and the stores).
+// 40560 x 8960 x 1536: 332 us bf16, 400 with GELU, 414 to 428 with the GELU quantised, 459 fp32, 722 with a residual: with six
+// k-groups a tile the epilogue is a third of the time (its vector work and the stores).
 // Not better: four waves of 128 x 128 outputs (4.3 PFLOP/s, a longer epilogue); 128 x 256 tiles in two workgroups per CU
 // (long K 3.8 PFLOP/s; short K with GELU 406 us against 421 then); the closing barriers ahead of a phase's last products
 // (2000 x 5120 x 5120 36.5 us against 34: the next reads wait behind them).

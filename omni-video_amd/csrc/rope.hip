@@ -7,7 +7,10 @@
 //   (x0, x1) -> (x0 c - x1 s, x0 s + x1 c),  pairs (2p, 2p + 1) or (p, p + D/2).
 //
 // The angle is a 64-bit product reduced to a quarter turn in 64 bits, then sine and cosine by their Taylor polynomials in
-// 32 bits (|r| <= pi/4: truncation below 2e-9): positions of any size cost no accuracy and there is no table to outgrow.
+// 32 bits (|r| <= pi/4: truncation below 2e-9).  The roundings of the frequency and of the product move an angle by at most
+// 2^-51 of the turns that it has made: below 2e-7 turns for every int32 position, and there is no table to outgrow; fp32
+// positions go further, and lose all meaning from about 1e15 on.  The rotation itself is fp32: 2^-20 of |x0| + |x1| at most,
+// then the rounding to x's type.
 // HBM-bound (every element read and written once): a lane owns 8 (bf16, fp32 alike) values of a head, computes the
 // turns of its pairs once per token and applies them to every head of the token that falls to it.  56640 tokens x 12 heads
 // of 128, bf16: 65 us = 5.3 TB/s.

@@ -1,7 +1,7 @@
 """Linear layers on MXFP4 operands (OCP microscaling: 4-bit E2M1 elements, one power-of-two scale per 32 consecutive
 values of a row): an extension beside the e4m3 mode, for layers the reference runs as bf16 nn.Linear
-(omnivideo/modules/model.py:125-154, :159-179, :218-258).  Backed by ovd_mxfp4_quant, ovd_mxfp4_dequant and
-ovd_gemm_mxfp4.  Inference only: the results carry no gradient."""
+(omnivideo/modules/model.py:125-154, :159-179, :218-258).  Backed by ovd_mxfp4_quant, ovd_mxfp4_dequant,
+ovd_gemm_mxfp4_as_rows and ovd_linear_mxfp4.  Inference only: the results carry no gradient."""
 import torch
 
 from .. import _hip as H

@@ -66,7 +66,9 @@ def packed_rope(x, positions, plan, out=None, inverse=False):
     """x [T, N, D] bf16 or fp32 (dense heads; the tokens may be strided), positions [T, axes] int32 or fp32 (or [T] for
     one axis), plan a RopePlan of head_dim D.  Returns the rotated heads, in `out` if given (x itself, or memory that does
     not overlap it).
-    inverse: the opposite rotation.  Positions may be of any size; results are rounded once, to x's type."""
+    inverse: the opposite rotation.  Angles are formed in 64 bits: off by at most 2^-51 of the turns made (2e-7 turns for any
+    int32 position; fp32 positions past about 1e15 mean nothing any more).  The rotation is computed in fp32 (2^-20 of
+    |x0| + |x1|) and rounded to x's type."""
     _no_grad(x)
     if positions.dim() == 1:
         positions = positions[:, None]
@@ -88,7 +90,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, max_q=None, max_k=None, causal=Fa
     cu_q, cu_k: int32 [documents + 1] device tensors; document d owns query rows cu_q[d] .. cu_q[d + 1] and key rows
     cu_k[d] .. cu_k[d + 1] (cu_k None: the same).  Query i of Lq sees the Lk keys of its document, with `causal` the
     first max(i + Lk - Lq + 1, prefix[d]) of them (prefix int32 [documents] or None).  softcap > 0 caps the scores:
-    softcap * tanh(s / softcap).  softmax_scale defaults to D ** -0.5.
+    softcap * tanh(s / softcap), exact to 2^-20 of a cap up to 256 and to 2^-18 of the score above.  softmax_scale defaults to
+    D ** -0.5.  Softmax and sums are fp32; the probabilities are rounded to bf16 for their product with v.
     A query that sees no key gets zeros.  Rows outside every document are not written (uninitialised when `out` is not
     given).  A key that is hidden from a query does not enter its result, whatever it and its value hold.  `out` may be q
     itself, but not share memory with k or v.
